@@ -390,6 +390,95 @@ PXQ_API int pxq_attention(const float* q, size_t q_rows, const float* k, const f
                           size_t kv_heads, size_t head_dim, const pxq_attention_range* ranges, size_t nranges,
                           size_t query_offset, float* output, void* stream);
 
+/* ---- attention over an 8-bit key/value cache ----------------------------
+ * No counterpart in the reference (its attention takes fp32 keys and values,
+ * src/tensor.cpp:347-427).  A cache holds, for each of `sequences` sequences,
+ * up to `capacity` tokens of kv_heads x head_dim keys and values in 8 bits,
+ * in blocks of PXQ_KV_BLOCK tokens with one fp32 scale for each (block,
+ * key/value head), K and V apart.  X being K or V, with A the largest |X|
+ * among the block's present tokens and channels:
+ *   d = fl32(A / 127);  q = the integer nearest to X / d, ties to even;
+ *   the cache stands for fl32(q * d)
+ * (d = 0 when A < 2^-118; when some |X| is not finite, d is NaN and so are all
+ * values of the block).  The rows of a sequence's last block are also kept in
+ * fp32 and the block is quantized anew as it fills, so what the cache holds
+ * depends on the rows alone, not on how they were cut into appends.
+ *
+ * The lengths live on the device: a captured step advances them on every
+ * replay.  Calls that write a cache (append, truncate, evict into it) must be
+ * ordered against every other call on it; calls that read one may overlap.
+ * Errors that only the device can see (bounds outside the arrays, an append
+ * beyond the capacity) leave the cache as it was and are reported by
+ * pxq_synchronize as PXQ_ERR_DEVICE_STATUS.
+ *
+ * Rows of a batch are packed: `starts` (device int32, sequences + 1 values,
+ * ascending) says that rows [starts[s], starts[s + 1]) are sequence s's; NULL:
+ * rows / sequences each, in order.  Rows past starts[sequences] are not
+ * touched. */
+typedef struct pxq_kv_cache pxq_kv_cache;
+#define PXQ_KV_BLOCK 32
+
+/* Device bytes that a cache needs (0: sizes it does not handle). */
+PXQ_API uint64_t pxq_kv_cache_bytes(size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim);
+
+/* An empty cache in `memory` (device, pxq_kv_cache_bytes() bytes, 256-byte
+ * aligned), which stays the caller's and outlives the cache.  head_dim 64, 80
+ * or 128; at most 1024 sequences, 4096 key/value heads, 2^30 tokens. */
+PXQ_API int pxq_kv_cache_create(void* memory, size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim,
+                                pxq_kv_cache** out, void* stream);
+/* Forget the cache (a host-side step: the memory is not touched). */
+PXQ_API int pxq_kv_cache_release(pxq_kv_cache* c);
+
+/* The sequences' lengths into `lengths` (device int32, sequences values). */
+PXQ_API int pxq_kv_cache_lengths(const pxq_kv_cache* c, int32_t* lengths, void* stream);
+
+/* Append rows of k and v (device fp32, row strides ldk, ldv >= kv_heads *
+ * head_dim floats: slices of a fused projection's output will do).  Bounds
+ * outside [0, rows] drop the whole call; a sequence whose rows would exceed
+ * the capacity keeps what it had. */
+PXQ_API int pxq_kv_append(pxq_kv_cache* c, const float* k, size_t ldk, const float* v, size_t ldv, size_t rows,
+                          const int32_t* starts, void* stream);
+
+/* Shorten every sequence s to lengths[s] tokens (device int32; NULL: 0).  A
+ * value that is negative or not below the present length leaves the sequence
+ * as it is.  Going back within the last block is exact; a block that was
+ * closed is opened again from the values it stands for. */
+PXQ_API int pxq_kv_truncate(pxq_kv_cache* c, const int32_t* lengths, void* stream);
+
+/* The values the cache stands for: tokens [first[s], first[s] + count) of
+ * every sequence (first: device int32, NULL: 0) into k and v (device fp32
+ * [sequences][count][kv_heads * head_dim]; either may be NULL).  Rows of
+ * tokens past a sequence's length are not written. */
+PXQ_API int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t count, float* k, float* v, void* stream);
+
+/* Attention of q's rows (device fp32, stride ldq) over the cache: pxq_attention
+ * on the values the cache stands for, to fp32 accuracy.  Sequence s has n =
+ * starts[s + 1] - starts[s] <= max_rows rows (max_rows is ignored without
+ * starts); causal: they are its last n tokens, row i sees the first
+ * len - n + i + 1 of them; otherwise every row sees all len.  A row that sees
+ * nothing gets zeros.  Rows of a sequence with bounds outside the arrays or more
+ * than max_rows rows are not written (a device-side error, as above).
+ * weights_out (may be NULL): [sequences][kv_heads][capacity], the attention
+ * weight that each cached token received from the rows and the heads that
+ * share its kv head, added to `weights` (same shape; NULL: zeros; may be
+ * weights_out itself).  Entries past a sequence's length are not touched.
+ * heads must be a multiple of the cache's kv_heads. */
+PXQ_API int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t rows, const int32_t* starts,
+                             size_t max_rows, size_t heads, int causal, float* output, size_t ldo, const float* weights,
+                             float* weights_out, void* stream);
+
+/* Evict: dst (same sequences, heads and head size, another cache) receives,
+ * for every sequence and key/value head of src, its last `recent` tokens and
+ * the keep - recent others of the largest weights ([sequences][kv_heads][src
+ * capacity]; ties: the lower index; NaN counts as -infinity), in their order,
+ * as if appended to an empty sequence; a sequence of at most `keep` tokens
+ * goes over whole.  weights_out (may be NULL): [sequences][kv_heads][dst
+ * capacity], the kept tokens' weights; kept (may be NULL): int32
+ * [sequences][kv_heads][keep], their places in src.  recent <= keep <= dst's
+ * capacity.  Entries past the new length are not touched. */
+PXQ_API int pxq_kv_evict(const pxq_kv_cache* src, pxq_kv_cache* dst, const float* weights, size_t keep, size_t recent,
+                         float* weights_out, int32_t* kept, void* stream);
+
 /* ---- GGUF model files: the format step in front of the upload ---------- */
 
 /* A GGUF v3 file mapped read-only, its tensor directory parsed with the

@@ -22,6 +22,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -1309,6 +1310,207 @@ int pxq_attention(const float* q, size_t q_rows, const float* k, const float* v,
     return PXQ_OK;
 }
 
+}  // extern "C"
+
+// ---- 8-bit key/value cache (kv_cache.cu, kv_attention.cu) --------------------
+struct pxq_kv_cache {
+    KvView v;
+    int device = 0;
+};
+
+namespace {
+
+int check_kv_sizes(size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim)
+{
+    if (!sequences || !capacity || !kv_heads || !head_dim) return fail(PXQ_ERR_INVALID, "zero size");
+    if (head_dim != 64 && head_dim != 80 && head_dim != 128)
+        return fail(PXQ_ERR_UNSUPPORTED, "head size %zu (64, 80 and 128 are handled)", head_dim);
+    if (sequences > (size_t)kKvMaxSequences)
+        return fail(PXQ_ERR_UNSUPPORTED, "%zu sequences (at most %d)", sequences, kKvMaxSequences);
+    if (kv_heads > 4096) return fail(PXQ_ERR_UNSUPPORTED, "%zu key/value heads (at most 4096)", kv_heads);
+    if (capacity > ((size_t)1 << 30)) return fail(PXQ_ERR_UNSUPPORTED, "capacity %zu (at most 2^30 tokens)", capacity);
+    if (sequences * kv_heads * ((capacity + kKvBlock - 1) / kKvBlock) > 0x7fffffffu)
+        return fail(PXQ_ERR_UNSUPPORTED, "more than 2^31 - 1 blocks");
+    return PXQ_OK;
+}
+
+int check_kv(const pxq_kv_cache* c)
+{
+    if (!c) return fail(PXQ_ERR_INVALID, "null cache");
+    if (c->device != t_device) return fail(PXQ_ERR_INVALID, "the cache is on device %d, the calling thread's is %d", c->device, t_device);
+    return PXQ_OK;
+}
+
+// The packed rows of a batch: with no starts, every sequence has the same number.
+int check_kv_rows(const pxq_kv_cache* c, size_t rows, const int32_t* starts)
+{
+    if (!rows) return fail(PXQ_ERR_INVALID, "no rows");
+    if (rows > 0x7fffffffu) return fail(PXQ_ERR_UNSUPPORTED, "%zu rows exceed INT32_MAX", rows);
+    if (!starts && rows % (size_t)c->v.S)
+        return fail(PXQ_ERR_INVALID, "%zu rows do not divide into %d sequences (give their starts)", rows, c->v.S);
+    return PXQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t pxq_kv_cache_bytes(size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim)
+{
+    if (check_kv_sizes(sequences, capacity, kv_heads, head_dim)) return 0;
+    return kv_layout((int64_t)sequences, (int64_t)kv_heads, (int64_t)head_dim, (int64_t)capacity, nullptr, nullptr);
+}
+
+int pxq_kv_cache_create(void* memory, size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim, pxq_kv_cache** out,
+                        void* stream)
+{
+    if (int rc = check_kv_sizes(sequences, capacity, kv_heads, head_dim)) return rc;
+    if (!memory || !out) return fail(PXQ_ERR_INVALID, "null memory or out");
+    if (reinterpret_cast<uintptr_t>(memory) % 256) return fail(PXQ_ERR_INVALID, "the cache's memory is not 256-byte aligned");
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    pxq_kv_cache* c = new (std::nothrow) pxq_kv_cache;
+    if (!c) return fail(PXQ_ERR_NO_MEMORY, "no host memory");
+    c->device = t_device;
+    kv_layout((int64_t)sequences, (int64_t)kv_heads, (int64_t)head_dim, (int64_t)capacity, static_cast<uint8_t*>(memory), &c->v);
+    const cudaError_t e = cudaMemsetAsync(memory, 0, 256 + sequences * 12, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) {
+        delete c;
+        return fail(PXQ_ERR_CUDA, "cannot clear the cache: %s", cudaGetErrorString(e));
+    }
+    *out = c;
+    return PXQ_OK;
+}
+
+int pxq_kv_cache_release(pxq_kv_cache* c)
+{
+    if (!c) return fail(PXQ_ERR_INVALID, "null cache");
+    delete c;
+    return PXQ_OK;
+}
+
+int pxq_kv_cache_lengths(const pxq_kv_cache* c, int32_t* lengths, void* stream)
+{
+    DeviceCtx* d;
+    if (!c || !lengths) return fail(PXQ_ERR_INVALID, "null cache or lengths");
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(c)) return rc;
+    PXQ_CUDA(cudaMemcpyAsync(lengths, c->v.lens, (size_t)c->v.S * 4, cudaMemcpyDeviceToDevice, static_cast<cudaStream_t>(stream)));
+    return PXQ_OK;
+}
+
+int pxq_kv_append(pxq_kv_cache* c, const float* k, size_t ldk, const float* v, size_t ldv, size_t rows, const int32_t* starts,
+                  void* stream)
+{
+    if (!c || !k || !v) return fail(PXQ_ERR_INVALID, "null cache, k or v");
+    const size_t width = (size_t)c->v.H * c->v.D;
+    if (ldk < width || ldv < width) return fail(PXQ_ERR_INVALID, "row stride below kv_heads * head_dim = %zu", width);
+    if (int rc = check_kv_rows(c, rows, starts)) return rc;
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(c)) return rc;
+    PXQ_CUDA(counted(launch_kv_append(c->v, k, (int64_t)ldk, v, (int64_t)ldv, (int64_t)rows, starts, d->status,
+                                      static_cast<cudaStream_t>(stream))));
+    return PXQ_OK;
+}
+
+int pxq_kv_truncate(pxq_kv_cache* c, const int32_t* lengths, void* stream)
+{
+    if (!c) return fail(PXQ_ERR_INVALID, "null cache");
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(c)) return rc;
+    PXQ_CUDA(counted(launch_kv_truncate(c->v, lengths, static_cast<cudaStream_t>(stream))));
+    return PXQ_OK;
+}
+
+int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t count, float* k, float* v, void* stream)
+{
+    if (!c || (!k && !v)) return fail(PXQ_ERR_INVALID, "null cache, or neither k nor v");
+    if (!count) return fail(PXQ_ERR_INVALID, "no tokens");
+    if (count > 0x7fffffffu) return fail(PXQ_ERR_UNSUPPORTED, "%zu tokens exceed INT32_MAX", count);
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(c)) return rc;
+    PXQ_CUDA(counted(launch_kv_read(c->v, first, (int64_t)count, k, v, static_cast<cudaStream_t>(stream))));
+    return PXQ_OK;
+}
+
+int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t rows, const int32_t* starts, size_t max_rows,
+                     size_t heads, int causal, float* output, size_t ldo, const float* weights, float* weights_out, void* stream)
+{
+    if (!c || !q || !output) return fail(PXQ_ERR_INVALID, "null cache, q or output");
+    if (!heads || heads % (size_t)c->v.H) return fail(PXQ_ERR_INVALID, "%zu heads over %d key/value heads", heads, c->v.H);
+    if (heads > 65535) return fail(PXQ_ERR_UNSUPPORTED, "%zu heads (at most 65535)", heads);
+    const size_t width = heads * (size_t)c->v.D;
+    if (ldq < width || ldo < width) return fail(PXQ_ERR_INVALID, "row stride below heads * head_dim = %zu", width);
+    if (weights && !weights_out) return fail(PXQ_ERR_INVALID, "weights without weights_out");
+    if (int rc = check_kv_rows(c, rows, starts)) return rc;
+    if (!starts) max_rows = rows / (size_t)c->v.S;
+    if (!max_rows || max_rows > rows) return fail(PXQ_ERR_INVALID, "max_rows %zu outside [1, rows = %zu]", max_rows, rows);
+    if (max_rows * (heads / (size_t)c->v.H) > 0x7fffffffu) return fail(PXQ_ERR_UNSUPPORTED, "rows x heads per group exceed INT32_MAX");
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(c)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    KvAttnCall a{};
+    a.c = c->v;
+    a.q = q;
+    a.out = output;
+    a.ldq = (int64_t)ldq;
+    a.ldo = (int64_t)ldo;
+    a.rows = (int64_t)rows;
+    a.starts = starts;
+    a.max_rows = (int64_t)max_rows;
+    a.heads = (int)heads;
+    a.causal = causal ? 1 : 0;
+    a.weights = weights;
+    a.weights_out = weights_out;
+    a.status = d->status;
+    // stream-ordered scratch: a captured call gets memory of its own graph
+    void* scratch = nullptr;
+    const size_t need = kv_attention_scratch_bytes(a, d->sms);
+    if (cudaMallocAsync(&scratch, need, s) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(PXQ_ERR_NO_MEMORY, "attention scratch of %zu bytes", need);
+    }
+    int launches = 0;
+    const cudaError_t e = launch_kv_attention(a, scratch, d->sms, s, &launches);
+    cudaFreeAsync(scratch, s);
+    if (counted(e, (uint64_t)launches) != cudaSuccess) return fail(PXQ_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    return PXQ_OK;
+}
+
+int pxq_kv_evict(const pxq_kv_cache* src, pxq_kv_cache* dst, const float* weights, size_t keep, size_t recent, float* weights_out,
+                 int32_t* kept, void* stream)
+{
+    if (!src || !dst || !weights) return fail(PXQ_ERR_INVALID, "null cache or weights");
+    if (src == dst || src->v.codes == dst->v.codes) return fail(PXQ_ERR_INVALID, "the destination is the source");
+    if (src->v.S != dst->v.S || src->v.H != dst->v.H || src->v.D != dst->v.D)
+        return fail(PXQ_ERR_INVALID, "the destination's sequences, heads or head size differ from the source's");
+    if (!keep || keep > (size_t)dst->v.cap) return fail(PXQ_ERR_INVALID, "keep %zu outside [1, the destination's capacity %d]", keep, dst->v.cap);
+    if (recent > keep) return fail(PXQ_ERR_INVALID, "recent %zu exceeds keep %zu", recent, keep);
+    if (weights_out == weights) return fail(PXQ_ERR_INVALID, "weights_out is weights");
+    DeviceCtx* d;
+    if (int rc = ensure_device(&d)) return rc;
+    if (int rc = check_kv(src)) return rc;
+    if (int rc = check_kv(dst)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    void* own = nullptr;
+    if (!kept) {
+        const size_t need = (size_t)src->v.S * src->v.H * keep * sizeof(int32_t);
+        if (cudaMallocAsync(&own, need, s) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(PXQ_ERR_NO_MEMORY, "eviction scratch of %zu bytes", need);
+        }
+    }
+    const cudaError_t e = launch_kv_evict(src->v, dst->v, weights, (int64_t)keep, (int64_t)recent, weights_out,
+                                          own ? static_cast<int32_t*>(own) : kept, s);
+    if (own) cudaFreeAsync(own, s);
+    if (counted(e, 2) != cudaSuccess) return fail(PXQ_ERR_CUDA, "eviction launch failed: %s", cudaGetErrorString(e));
+    return PXQ_OK;
+}
+
 int pxq_gemm_block_dots(pxq_weight* w, size_t row_first, size_t row_count, const float* input, size_t columns, float* dump,
                         void* stream)
 {
@@ -1369,6 +1571,8 @@ int pxq_synchronize(void* stream)
         cudaDeviceSynchronize();
         reset_scratch_counters(t_device);
         cudaMemset(d->status, 0, 4);
+        if (st == kDevKvStarts) return fail(PXQ_ERR_DEVICE_STATUS, "key/value cache: row bounds outside the arrays or above max_rows");
+        if (st == kDevKvCapacity) return fail(PXQ_ERR_DEVICE_STATUS, "key/value cache: an append exceeded the capacity and was dropped");
         return fail(PXQ_ERR_DEVICE_STATUS, "a kernel gave up waiting (status %u); scratch counters reset", st);
     }
     return PXQ_OK;

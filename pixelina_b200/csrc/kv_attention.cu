@@ -1,0 +1,562 @@
+// kv_attention.cu -- softmax attention over the 8-bit key/value cache
+// (kv_cache.cuh), and the weight that each cached token receives.
+//
+// Query row i of a sequence with n rows and len tokens sees the tokens
+// j < L(i) = len (or len - n + i + 1 when causal):
+//     z_j = (q . k_j) dk / sqrt(D),  p_j = exp(z_j - max) / sum,  out = sum_j p_j dv v_j
+// with k, v the codes and dk, dv their blocks' scales; L <= 0 gives zeros.
+// A pair is (query row, head of the kv head's group): pairs p = i * G + g are
+// the rows of the matrix products, so every key is read once for the group.
+//
+// Accuracy: codes are exact in fp16.  q (scaled per pair by a power of two to
+// below 2^15) and p are each the sum of two fp16 numbers, hi + lo, which
+// leaves 2^-22 of the value; products and sums are fp32.  So the result is
+// that of an fp32 computation at two half-precision products per element.
+//
+//   k_kv_attn     split keys: one CTA per SM takes an equal run of the
+//                 flattened (sequence, head, block) list; warps take a run's
+//                 blocks in turn, each with its own running max and sum
+//   k_kv_combine  joins the parts of a (sequence, head) that spans CTAs
+//   k_kv_weights  the weights, from each pair's max and sum
+#include <algorithm>
+#include <type_traits>
+#include "kv_cache.cuh"
+
+namespace pxq {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int AW = 8;                    // warps per CTA
+constexpr int kMinRun = 8;               // fewest blocks worth a CTA: one per warp
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^e for -126 <= e <= 127
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 126; }  // |x| < 2^this
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (a, b) = hi + lo, each half of the packed words
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack_half2(a - f.x, b - f.y);
+}
+
+// D += A (16 x 16, row) * B (16 x 8, column), fp16 in, fp32 out
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct AttnParams {
+    KvAttnCall a;
+    float* part;   // partial results: [pair tile][CTA][2] x {m[PT], l[PT], O[PT][D]}
+    float* lse;    // [rows][heads] log2 of the softmax's denominator with its max, when weights are wanted
+    int runs;      // CTAs of the flattened list
+};
+
+// Blocks of sequence s: 0 when it has no rows to answer.  An empty cache
+// counts one (fully masked) block, so that its rows get their zeros.
+__device__ __forceinline__ int kv_attn_blocks(const KvAttnCall& a, int s)
+{
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    if (q.n <= 0 || q.n > a.max_rows) return 0;
+    return max(1, (q.len + kKvBlock - 1) / kKvBlock);
+}
+__device__ __forceinline__ int kv_run_length(int total, int runs) { return max(kMinRun, (total + runs - 1) / runs); }
+
+// Tokens that pair p's row sees.
+__device__ __forceinline__ int kv_limit(const KvAttnCall& a, const KvSeq& q, int i)
+{
+    return a.causal ? max(0, q.len - q.n + i + 1) : q.len;
+}
+
+// One warp's A fragments of up to PT pairs' queries: PT = 8 packs hi into
+// rows 0-7 and lo into rows 8-15 of one fragment, PT = 16 keeps two.
+// coef[r]: log2(e) / sqrt(D) over the pair's power of two.
+template <int D, int PT>
+struct QFrag {
+    uint32_t hi[D / 16][4];
+    uint32_t lo[PT == 16 ? D / 16 : 1][4];
+    float coef[PT / 8];
+
+    __device__ __forceinline__ void load(const KvAttnCall& a, const KvSeq& q, int h, int tile)
+    {
+        const int lane = lane_id(), r = lane / 4, c = lane % 4, G = a.heads / a.c.H, pairs = q.n * G;
+#pragma unroll
+        for (int u = 0; u < PT / 8; u++) {
+            const int p = tile * PT + r + 8 * u;
+            const bool live = p < pairs;
+            const float* src = a.q + (int64_t)(q.row0 + (live ? p / G : 0)) * a.ldq + (int64_t)(h * G + (live ? p % G : 0)) * D;
+            float m = 0.f;
+            float x[D / 16][4];
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                const int d = k < D / 64 * 4 ? 64 * (k / 4) + 16 * c + 4 * (k % 4) : D / 64 * 64 + 4 * c;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[k][i] = live ? src[d + i] : 0.f;
+                    m = fmaxf(m, fabsf(x[k][i]));
+                }
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            // |x| 2^e < 2^15; a row of zeros, or one that is not finite, stays as it is
+            const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - exponent_of(m))) : 0;
+            const float up = pow2i(e);
+            coef[u] = kLog2E / sqrtf((float)D) * pow2i(-e);
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                uint32_t h0, l0, h1, l1;
+                split_half2(x[k][0] * up, x[k][1] * up, h0, l0);
+                split_half2(x[k][2] * up, x[k][3] * up, h1, l1);
+                if (PT == 8) {
+                    hi[k][0] = h0, hi[k][1] = l0, hi[k][2] = h1, hi[k][3] = l1;
+                } else {
+                    hi[k][u] = h0, hi[k][2 + u] = h1;
+                    lo[k][u] = l0, lo[k][2 + u] = l1;
+                }
+            }
+        }
+    }
+};
+
+// Scores of a block's 32 tokens: z[u][8] of pair row r + 8 u, tokens 8 c ..
+// 8 c + 7, before the scales.  rec: the block's record.
+template <int D, int PT>
+__device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_t* rec, float (&z)[PT / 8][8])
+{
+    constexpr int J = D / 64;
+    const int lane = lane_id();
+    float s[4][4];
+#pragma unroll
+    for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[nt][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            const uint4 w = *reinterpret_cast<const uint4*>(rec + ((nt * J + j) * 32 + lane) * 16);
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t b0 = kv_half2_lo(ww[k]), b1 = kv_half2_hi(ww[k]);
+                mma16816(s[nt], q.hi[4 * j + k], b0, b1);
+                if (PT == 16) mma16816(s[nt], q.lo[4 * j + k], b0, b1);
+            }
+        }
+    }
+    if (D % 64 != 0) {
+        const uint4 w = *reinterpret_cast<const uint4*>(rec + 32 * 64 * J + lane * 16);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            const uint32_t b0 = kv_half2_lo(ww[nt]), b1 = kv_half2_hi(ww[nt]);
+            mma16816(s[nt], q.hi[4 * J], b0, b1);
+            if (PT == 16) mma16816(s[nt], q.lo[PT == 16 ? 4 * J : 0], b0, b1);
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (PT == 8) {
+                z[0][2 * nt + e] = s[nt][e] + s[nt][2 + e];
+            } else {
+                z[0][2 * nt + e] = s[nt][e];
+                z[PT / 8 - 1][2 * nt + e] = s[nt][2 + e];
+            }
+        }
+}
+
+constexpr int kAttnStages = 3;  // blocks in flight per warp
+template <int D>
+constexpr size_t attn_smem_bytes() { return (size_t)AW * kAttnStages * kv_record_bytes(D); }
+
+template <int D, int PT>
+__global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ AttnParams P)
+{
+    constexpr int NST = kAttnStages, REC = kv_record_bytes(D), U = PT / 8, NT = D / 8;
+    constexpr int CW = NST * REC / 4;  // floats between two warps' rings
+    static_assert(PT * (D + 2) <= CW, "a warp's result fits its ring");
+    extern __shared__ __align__(128) uint8_t dyn[];
+    __shared__ int sum[kKvMaxSequences + 1];
+    __shared__ int warp_sums[32];
+    __shared__ uint64_t bars[AW][NST];
+    __shared__ uint32_t abort_flag;
+    const KvAttnCall& a = P.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane / 4, c = lane % 4;
+    const int tile = blockIdx.y, G = a.heads / a.c.H;
+    uint8_t* ring = dyn + warp * NST * REC;
+    float* comb = reinterpret_cast<float*>(dyn);  // at a segment's end, in each warp's ring: m[PT], l[PT], O[PT][D]
+    if (tid == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int i = 0; i < NST; i++) mbar_init(&bars[warp][i], 1);
+        fence_mbar_init();
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
+        const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
+        return kv_attn_blocks(a, s) * a.c.H;
+    });
+    const int total = sum[a.c.S], run = kv_run_length(total, P.runs);
+    const int w0 = (int)blockIdx.x * run, w1 = min(total, w0 + run);
+    uint32_t phase = 0;  // bit i: parity of stage i
+
+    for (int w = w0; w < w1;) {
+        const int s = kv_find(sum, a.c.S, w);
+        const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+        const int nb = kv_attn_blocks(a, s);
+        const int h = (w - sum[s]) / nb, seg = sum[s] + h * nb;  // this (sequence, head)'s blocks: [seg, seg + nb)
+        const int b0 = w - seg, b1 = min(seg + nb, w1) - seg;
+        const bool first = b0 > 0, whole = b0 == 0 && b1 == nb;
+        w = seg + b1;
+        const int pairs = q.n * G;
+        if (tile * PT >= pairs) continue;
+        const uint8_t* recs = a.c.codes + ((int64_t)s * a.c.H + h) * a.c.nb * (int64_t)REC;
+        const float2* scales = a.c.scales + ((int64_t)s * a.c.H + h) * a.c.nb;
+
+        int issued = b0 + warp;
+        auto issue = [&](int st) {
+            if (lane == 0 && issued < b1) {
+                mbar_expect_tx(&bars[warp][st], REC);
+                bulk_load(ring + st * REC, recs + (int64_t)issued * REC, REC, &bars[warp][st]);
+            }
+            issued += AW;
+        };
+#pragma unroll
+        for (int i = 0; i < NST; i++) issue(i);
+
+        // after a timeout: give the copies still in flight a last, bounded chance to land
+        auto drain = [&](int b, int st) {
+            for (; b < min(issued, b1); b += AW, st = st + 1 == NST ? 0 : st + 1)
+                for (int i = 0; i < 1000 && !mbar_try_wait(&bars[warp][st], (phase >> st) & 1u); i++) {}
+        };
+
+        QFrag<D, PT> qf;
+        qf.load(a, q, h, tile);
+        int lim[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = tile * PT + r + 8 * u;
+            lim[u] = p < pairs ? kv_limit(a, q, p / G) : 0;
+        }
+        float m[U], l[U], o[NT][4];
+        int E = -100;  // o is in units of 2^(E - 15); smaller scales lose nothing that fp32 sums would keep
+#pragma unroll
+        for (int u = 0; u < U; u++) m[u] = -INFINITY, l[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] = 0.f;
+
+        int st = 0;
+        float2 next = b0 + warp < b1 ? scales[b0 + warp] : make_float2(0.f, 0.f);
+        for (int b = b0 + warp; b < b1; b += AW) {
+            const float2 sc = next;
+            if (b + AW < b1) next = scales[b + AW];
+            if (!mbar_wait(&bars[warp][st], (phase >> st) & 1u, &abort_flag, a.status, kDevTimeoutFull)) {
+                drain(b, st);
+                break;
+            }
+            phase ^= 1u << st;
+            const uint8_t* rec = ring + st * REC;
+            float z[U][8];
+            block_scores<D, PT>(qf, rec, z);
+            // online softmax; lane (r, c) holds tokens 32 b + 8 c .. + 7 of its pairs
+            const int t0 = kKvBlock * b + 8 * c;
+            uint32_t ph[U][4], pl[U][4];
+            const int ev = exponent_of(sc.y);
+            const int En = ev < 129 ? max(E, ev) : E;  // a NaN scale has exponent 129
+            const float up = sc.y * pow2i(15 - En);
+            float corr[U];
+            bool moved = En != E;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float k = qf.coef[u] * sc.x;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    z[u][i] *= k;
+                    if (t0 + i >= lim[u]) z[u][i] = -INFINITY;
+                    mx = fmaxf(mx, z[u][i]);
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.f : mn;
+                corr[u] = ex2(m[u] - ms);
+                moved |= mn != m[u];
+                m[u] = mn;
+                float add = 0.f, y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = ex2(z[u][i] - ms);
+                    add += p;
+                    y[i] = t0 + i < lim[u] ? p * up : 0.f;
+                }
+                l[u] = l[u] * corr[u] + add;
+#pragma unroll
+                for (int i = 0; i < 4; i++) split_half2(y[2 * i], y[2 * i + 1], ph[u][i], pl[u][i]);
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+                const float ef = pow2i(max(-126, E - En));
+                E = En;
+                const float c0 = corr[0] * ef, c1 = PT == 8 ? c0 : corr[U - 1] * ef;
+#pragma unroll
+                for (int i = 0; i < NT; i++) o[i][0] *= c0, o[i][1] *= c0, o[i][2] *= c1, o[i][3] *= c1;
+            }
+            uint32_t ah[2][4], al[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                if (PT == 8) {
+                    ah[k][0] = ph[0][2 * k], ah[k][1] = pl[0][2 * k], ah[k][2] = ph[0][2 * k + 1], ah[k][3] = pl[0][2 * k + 1];
+                } else {
+                    ah[k][0] = ph[0][2 * k], ah[k][1] = ph[U - 1][2 * k], ah[k][2] = ph[0][2 * k + 1], ah[k][3] = ph[U - 1][2 * k + 1];
+                    al[k][0] = pl[0][2 * k], al[k][1] = pl[U - 1][2 * k], al[k][2] = pl[0][2 * k + 1], al[k][3] = pl[U - 1][2 * k + 1];
+                }
+            }
+#pragma unroll
+            for (int np = 0; np < D / 16; np++) {
+                const uint4 vw = *reinterpret_cast<const uint4*>(rec + 32 * D + (np * 32 + lane) * 16);
+                const uint32_t ww[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+                for (int f = 0; f < 2; f++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const uint32_t v0 = kv_half2_lo(ww[2 * f + k]), v1 = kv_half2_hi(ww[2 * f + k]);
+                        mma16816(o[2 * np + f], ah[k], v0, v1);
+                        if (PT == 16) mma16816(o[2 * np + f], al[k], v0, v1);
+                    }
+            }
+            __syncwarp();
+            issue(st);
+            if (++st == NST) st = 0;
+        }
+        // Join the warps, through the rings: every copy of the segment has been
+        // consumed, and each stage's phase bit is kept, so the next segment
+        // starts from stage 0 again.
+        float* mine = comb + warp * CW;
+        const float back = pow2i(E - 15);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+            if (c == 0) {
+                mine[r + 8 * u] = m[u];
+                mine[PT + r + 8 * u] = l[u];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            float* row = mine + 2 * PT + r * D + 8 * i + 2 * c;
+            if (PT == 8) {
+                row[0] = (o[i][0] + o[i][2]) * back;
+                row[1] = (o[i][1] + o[i][3]) * back;
+            } else {
+                row[0] = o[i][0] * back;
+                row[1] = o[i][1] * back;
+                row[8 * D] = o[i][2] * back;
+                row[8 * D + 1] = o[i][3] * back;
+            }
+        }
+        __syncthreads();
+        float* part = P.part + (((int64_t)tile * P.runs + blockIdx.x) * 2 + (first ? 0 : 1)) * PT * (D + 2);
+        for (int x = tid; x < PT * D; x += AW * 32) {
+            const int p = x / D, d = x % D, gp = tile * PT + p;
+            float M = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < AW; i++) M = fmaxf(M, comb[i * CW + p]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+            float L = 0.f, O = 0.f;
+#pragma unroll
+            for (int i = 0; i < AW; i++) {
+                const float* src = comb + i * CW;
+                const float f = ex2(src[p] - Ms);
+                L += src[PT + p] * f;
+                O += src[2 * PT + p * D + d] * f;
+            }
+            if (gp >= pairs) continue;
+            if (whole) {
+                const int64_t row = q.row0 + gp / G;
+                const int head = h * G + gp % G;
+                // no token seen: zeros.  The test is on the max, so that a NaN sum stays NaN.
+                a.out[row * a.ldo + (int64_t)head * D + d] = M == -INFINITY && L == 0.f ? 0.f : O / L;
+                if (P.lse && d == 0) P.lse[row * a.heads + head] = M == -INFINITY && L == 0.f ? INFINITY : M + log2f(L);
+            } else {
+                part[2 * PT + x] = O;
+                if (d == 0) {
+                    part[p] = M;
+                    part[PT + p] = L;
+                }
+            }
+        }
+        fence_proxy_async_smem();  // the next segment's copies follow these writes
+        __syncthreads();
+        if (abort_flag) return;
+    }
+}
+
+// Parts of a (sequence, head) that spans CTAs, in their order.  One CTA of
+// 128 threads per (pair, head, sequence).
+template <int D, int PT>
+__global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ AttnParams P)
+{
+    __shared__ int sum[kKvMaxSequences + 1];
+    __shared__ int warp_sums[32];
+    const KvAttnCall& a = P.a;
+    griddep_wait();
+    griddep_launch_dependents();
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * a.c.H; });
+    const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.heads / a.c.H;
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const int nb = (sum[s + 1] - sum[s]) / a.c.H;
+    if (nb == 0 || gp >= q.n * G) return;
+    const int run = kv_run_length(sum[a.c.S], P.runs), seg = sum[s] + h * nb;
+    const int c0 = seg / run, c1 = (seg + nb - 1) / run;
+    if (c0 == c1) return;  // written by the CTA that had all of it
+    const int tile = gp / PT, p = gp % PT;
+    auto part = [&](int cta) {
+        return P.part + (((int64_t)tile * P.runs + cta) * 2 + (cta == c0 && seg >= cta * run ? 1 : 0)) * PT * (D + 2);
+    };
+    float M = -INFINITY;
+    for (int i = c0; i <= c1; i++) M = fmaxf(M, part(i)[p]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+    for (int i = c0; i <= c1; i++) {
+        const float* src = part(i);
+        const float f = ex2(src[p] - Ms);
+        L += src[PT + p] * f;
+        if (d < D) O += src[2 * PT + p * D + d] * f;
+    }
+    const int64_t row = q.row0 + gp / G;
+    const int head = h * G + gp % G;
+    if (d < D) a.out[row * a.ldo + (int64_t)head * D + d] = M == -INFINITY && L == 0.f ? 0.f : O / L;
+    if (P.lse && d == 0) P.lse[row * a.heads + head] = M == -INFINITY && L == 0.f ? INFINITY : M + log2f(L);
+}
+
+// weights_out = weights + the p of every pair that sees the token.  One warp
+// per block of 32 tokens; a lane sums its 8 tokens over the pair tiles, then
+// the eight lanes that share them add up in a fixed order.
+template <int D>
+__global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ AttnParams P)
+{
+    const KvAttnCall& a = P.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
+    const int s = blockIdx.z, h = blockIdx.y, b = blockIdx.x * AW + warp, G = a.heads / a.c.H;
+    griddep_wait();
+    griddep_launch_dependents();
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    if (kKvBlock * (int64_t)b >= q.len) return;
+    const int64_t sh = (int64_t)s * a.c.H + h;
+    const uint8_t* rec = a.c.codes + (sh * a.c.nb + b) * kv_record_bytes(D);
+    const float dk = a.c.scales[sh * a.c.nb + b].x;
+    const int pairs = q.n > 0 && q.n <= a.max_rows ? q.n * G : 0, t0 = kKvBlock * b + 8 * c;
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = 0.f;
+    for (int tile = 0; tile * 8 < pairs; tile++) {
+        const int p = tile * 8 + r;
+        const int lim = p < pairs ? kv_limit(a, q, p / G) : 0;
+        if (!__any_sync(0xffffffffu, lim > kKvBlock * b)) continue;
+        QFrag<D, 8> qf;
+        qf.load(a, q, h, tile);
+        float z[1][8];
+        block_scores<D, 8>(qf, rec, z);
+        const float lse = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] += t0 + i < lim ? ex2(z[0][i] * (qf.coef[0] * dk) - lse) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], off);
+        if (r == i && t0 + i < q.len) {
+            const int64_t at = sh * a.c.cap + t0 + i;
+            a.weights_out[at] = (a.weights ? a.weights[at] : 0.f) + w[i];
+        }
+    }
+}
+
+template <typename F>
+cudaError_t by_dim(int D, F f)
+{
+    switch (D) {
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 80: return f(std::integral_constant<int, 80>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+struct AttnPlan {
+    int pt, tiles, runs;
+    size_t part_bytes, lse_bytes;
+};
+
+AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
+{
+    AttnPlan p{};
+    const int64_t pairs = a.max_rows * (a.heads / a.c.H);
+    p.pt = pairs <= 8 ? 8 : 16;
+    p.tiles = (int)((pairs + p.pt - 1) / p.pt);
+    p.runs = num_sms;
+    p.part_bytes = ((size_t)p.tiles * p.runs * 2 * p.pt * (a.c.D + 2) * sizeof(float) + 255) / 256 * 256;
+    p.lse_bytes = a.weights_out ? (size_t)a.rows * a.heads * sizeof(float) : 0;
+    return p;
+}
+
+template <int D, int PT>
+cudaError_t launch_split(const AttnParams& P, const AttnPlan& p, cudaStream_t s)
+{
+    constexpr size_t smem = attn_smem_bytes<D>();
+    cudaError_t e = cudaFuncSetAttribute(k_kv_attn<D, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_kv_attn<D, PT>, dim3((unsigned)p.runs, (unsigned)p.tiles), dim3(AW * 32), smem, s, P);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_kv_combine<D, PT>, dim3((unsigned)(P.a.max_rows * (P.a.heads / P.a.c.H)), (unsigned)P.a.c.H, (unsigned)P.a.c.S),
+                      dim3(128), 0, s, P);
+}
+
+}  // namespace
+
+size_t kv_attention_scratch_bytes(const KvAttnCall& a, int num_sms)
+{
+    const AttnPlan p = plan_kv(a, num_sms);
+    return p.part_bytes + p.lse_bytes;
+}
+
+cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms, cudaStream_t s, int* launches)
+{
+    const AttnPlan p = plan_kv(a, num_sms);
+    AttnParams P{};
+    P.a = a;
+    P.part = static_cast<float*>(scratch);
+    P.lse = p.lse_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.part_bytes) : nullptr;
+    P.runs = p.runs;
+    *launches = a.weights_out ? 3 : 2;
+    return by_dim(a.c.D, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        cudaError_t e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
+        if (e != cudaSuccess || !a.weights_out) return e;
+        return launch_pdl(k_kv_weights<D>, dim3((unsigned)((a.c.nb + AW - 1) / AW), (unsigned)a.c.H, (unsigned)a.c.S), dim3(AW * 32), 0,
+                          s, P);
+    });
+}
+
+}  // namespace pxq

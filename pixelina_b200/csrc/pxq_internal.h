@@ -174,6 +174,52 @@ cudaError_t launch_attention(const float* q, int64_t q_rows, const float* k, con
                              const int* range_causal, int nranges, int64_t query_offset, float* out, float* scratch,
                              size_t scratch_bytes, int num_sms, cudaStream_t s);
 
+// ---- kv_cache.cu -----------------------------------------------------------
+// The 8-bit key/value cache (layout: kv_cache.cuh) in the caller's memory.
+constexpr int kKvBlock = 32;          // tokens per block
+constexpr int kKvMaxSequences = 1024;
+// status codes beside those of pxq_device.cuh, which the host tells apart
+constexpr uint32_t kDevKvStarts = 8;    // row bounds outside the arrays, or more rows than announced
+constexpr uint32_t kDevKvCapacity = 9;  // an append beyond the capacity
+struct KvView {
+    int32_t* lens;     // [S] tokens held
+    int32_t* slot;     // [S] live tail slot
+    int32_t* held;     // [S] block whose rows that slot holds, -1: none
+    uint32_t* ticket;  // CTAs of the running append / truncate that are done
+    float2* scales;    // [S][H][nb] (K, V)
+    float* tail;       // [S][2][H][2][32][D]: slot, head, K / V
+    uint8_t* codes;    // [S][H][nb][64 * D]
+    int S, H, D, cap, nb;
+};
+// Bytes of a cache's memory; when `base` is given, fills in the view.
+size_t kv_layout(int64_t S, int64_t H, int64_t D, int64_t cap, uint8_t* base, KvView* v);
+cudaError_t launch_kv_append(const KvView& c, const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t rows,
+                             const int32_t* starts, uint32_t* status, cudaStream_t s);
+cudaError_t launch_kv_truncate(const KvView& c, const int32_t* lengths, cudaStream_t s);
+cudaError_t launch_kv_read(const KvView& c, const int32_t* first, int64_t count, float* k, float* v, cudaStream_t s);
+// weights [S][H][src.cap]; kept: int32 [S][H][keep], the source index of every kept token; weights_out
+// [S][H][dst.cap] or null
+cudaError_t launch_kv_evict(const KvView& src, const KvView& dst, const float* weights, int64_t keep, int64_t recent,
+                            float* weights_out, int32_t* kept, cudaStream_t s);
+
+// ---- kv_attention.cu -------------------------------------------------------
+struct KvAttnCall {
+    KvView c;
+    const float* q;
+    float* out;
+    int64_t ldq, ldo, rows;
+    const int32_t* starts;   // device [S + 1], or null: rows / S rows each
+    int64_t max_rows;        // most rows of one sequence
+    int heads;
+    int causal;
+    const float* weights;    // [S][H][cap] running totals, may be null (zero)
+    float* weights_out;      // null: no weights wanted
+    uint32_t* status;
+};
+size_t kv_attention_scratch_bytes(const KvAttnCall& a, int num_sms);
+// *launches: kernels launched
+cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms, cudaStream_t s, int* launches);
+
 // ---- shards.cu -------------------------------------------------------------
 cudaError_t launch_gather_shards(const float* src, int64_t shards, int64_t columns, int64_t shard_rows, float* dst,
                                  int64_t ldy, cudaStream_t s);

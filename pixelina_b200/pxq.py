@@ -20,6 +20,7 @@ without a B200 raises instead of falling back to any CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -95,6 +96,15 @@ SIGNATURES = {
     "pxq_sharded_matmul": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp]),
     "pxq_sharded_matmul_host": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _vp]),
     "pxq_attention": (_i, [_vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _vp]),
+    "pxq_kv_cache_bytes": (_u64, [_sz, _sz, _sz, _sz]),
+    "pxq_kv_cache_create": (_i, [_vp, _sz, _sz, _sz, _sz, C.POINTER(_vp), _vp]),
+    "pxq_kv_cache_release": (_i, [_vp]),
+    "pxq_kv_cache_lengths": (_i, [_vp, _vp, _vp]),
+    "pxq_kv_append": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp]),
+    "pxq_kv_truncate": (_i, [_vp, _vp, _vp]),
+    "pxq_kv_read": (_i, [_vp, _vp, _sz, _vp, _vp, _vp]),
+    "pxq_kv_attention": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _sz, _i, _vp, _sz, _vp, _vp, _vp]),
+    "pxq_kv_evict": (_i, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp]),
     "pxq_gguf_open": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "pxq_gguf_close": (_i, [_vp]),
     "pxq_gguf_tensor_count": (_sz, [_vp]),
@@ -298,6 +308,145 @@ def attention(q, k, v, heads: int, kv_heads: int, ranges=None, query_offset: int
     _check(load().pxq_attention(_ptr(q), rows, _ptr(k), _ptr(v), keys, heads, kv_heads, d, C.cast(arr, C.c_void_p), len(ranges),
                                 query_offset, _ptr(out), _stream_ptr(stream)))
     return out
+
+
+def _on(stream):
+    """Tensors made within belong to the stream that the call runs on."""
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+
+
+def _rows(x, width: int, what: str, device):
+    """An fp32 matrix of `width` columns on `device` whose rows may be strided."""
+    torch = _torch()
+    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != width or x.device != device:
+        raise ValueError(f"{what} must be fp32 [rows, {width}] on {device}")
+    return x if x.stride(1) == 1 and x.stride(0) >= width else x.contiguous()
+
+
+def _whole(x, shape, dtype, what: str, device):
+    """A contiguous tensor of this shape and type on `device`, or None."""
+    if x is not None and (tuple(x.shape) != tuple(shape) or x.dtype != dtype or not x.is_contiguous() or x.device != device):
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    return x
+
+
+def _ld(x) -> int:
+    """Row stride of a matrix (one row: its width, whatever torch says)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+class KVCache:
+    """An 8-bit key/value cache (pxq_kv_cache) for `sequences` sequences of up
+    to `capacity` tokens; its memory is a torch tensor of its own."""
+
+    def __init__(self, sequences: int, capacity: int, kv_heads: int, head_dim: int, stream=None):
+        torch = _torch()
+        lib = load()
+        nbytes = int(lib.pxq_kv_cache_bytes(sequences, capacity, kv_heads, head_dim))
+        if not nbytes:
+            raise PxqError(ERR_UNSUPPORTED, last_error())
+        self.sequences, self.capacity, self.kv_heads, self.head_dim = sequences, capacity, kv_heads, head_dim
+        with _on(stream):
+            self.memory = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        self.device = self.memory.device
+        h = C.c_void_p()
+        _check(lib.pxq_kv_cache_create(_ptr(self.memory), sequences, capacity, kv_heads, head_dim, C.byref(h), _stream_ptr(stream)))
+        self.handle = h
+
+    def release(self) -> None:
+        """Forget the cache; its memory goes back to torch."""
+        if self.handle:
+            _check(load().pxq_kv_cache_release(self.handle))
+            self.handle, self.memory = C.c_void_p(), None
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.pxq_kv_cache_release(self.handle)
+            self.handle = C.c_void_p()
+
+    def _live(self):
+        if not self.handle:
+            raise ValueError("the cache was released")
+        return self.handle
+
+    def _per_sequence(self, x, what: str, more: int = 0):
+        return _whole(x, (self.sequences + more,), _torch().int32, what, self.device)
+
+    def lengths(self, stream=None):
+        """The sequences' lengths: int32 cuda tensor."""
+        h = self._live()
+        with _on(stream):
+            out = _torch().empty(self.sequences, dtype=_torch().int32, device=self.device)
+        _check(load().pxq_kv_cache_lengths(h, _ptr(out), _stream_ptr(stream)))
+        return out
+
+    def append(self, k, v, starts=None, stream=None) -> None:
+        """Append rows k, v [rows, kv_heads*d]; rows [starts[s], starts[s+1]) go to sequence s."""
+        h = self._live()
+        width = self.kv_heads * self.head_dim
+        with _on(stream):
+            k, v = _rows(k, width, "k", self.device), _rows(v, width, "v", self.device)
+        if k.shape[0] != v.shape[0]:
+            raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
+        _check(load().pxq_kv_append(h, _ptr(k), _ld(k), _ptr(v), _ld(v), k.shape[0], _ptr(self._per_sequence(starts, "starts", 1)),
+                                    _stream_ptr(stream)))
+
+    def truncate(self, lengths=None, stream=None) -> None:
+        """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them)."""
+        _check(load().pxq_kv_truncate(self._live(), _ptr(self._per_sequence(lengths, "lengths")), _stream_ptr(stream)))
+
+    def read(self, first=None, count: Optional[int] = None, k=None, v=None, stream=None):
+        """The values of tokens [first[s], first[s] + count) of every sequence:
+        k, v [sequences, count, kv_heads*d].  Rows past a sequence's length are
+        not written (zeros in tensors made here)."""
+        torch = _torch()
+        h = self._live()
+        count = self.capacity if count is None else count
+        shape = (self.sequences, count, self.kv_heads * self.head_dim)
+        with _on(stream):
+            k, v = (torch.zeros(shape, device=self.device) if x is None else _whole(x, shape, torch.float32, what, self.device)
+                    for x, what in ((k, "k"), (v, "v")))
+        _check(load().pxq_kv_read(h, _ptr(self._per_sequence(first, "first")), count, _ptr(k), _ptr(v), _stream_ptr(stream)))
+        return k, v
+
+
+def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[int] = None, causal: bool = True, weights=None,
+                 weights_out=None, out=None, stream=None):
+    """Attention of q [rows, heads*d] over the cache (pxq_kv_attention): rows
+    [starts[s], starts[s+1]) are sequence s's, at most max_rows of them each
+    (None: no bound but rows).  weights_out = weights + what each cached token
+    received, [sequences, kv_heads, capacity]."""
+    torch = _torch()
+    h = cache._live()
+    width = heads * cache.head_dim
+    with _on(stream):
+        q = _rows(q, width, "q", cache.device)
+        rows = q.shape[0]
+        if out is None:
+            out = torch.empty((rows, width), dtype=torch.float32, device=cache.device)
+    if tuple(out.shape) != (rows, width) or out.dtype != torch.float32 or out.device != cache.device or out.stride(1) != 1 or _ld(out) < width:
+        raise ValueError(f"out must be fp32 [{rows}, {width}] on {cache.device}, its rows contiguous")
+    shape = (cache.sequences, cache.kv_heads, cache.capacity)
+    _whole(weights, shape, torch.float32, "weights", cache.device)
+    _whole(weights_out, shape, torch.float32, "weights_out", cache.device)
+    _check(load().pxq_kv_attention(h, _ptr(q), _ld(q), rows, _ptr(cache._per_sequence(starts, "starts", 1)), max_rows or rows, heads,
+                                   1 if causal else 0, _ptr(out), _ld(out), _ptr(weights), _ptr(weights_out), _stream_ptr(stream)))
+    return out
+
+
+def kv_evict(src: KVCache, dst: KVCache, weights, keep: Optional[int] = None, recent: int = 0, weights_out=None, kept=None,
+             stream=None) -> None:
+    """Into dst: the last `recent` tokens of src's every (sequence, kv head) and
+    the heaviest others, `keep` in all (None: dst's capacity) (pxq_kv_evict)."""
+    torch = _torch()
+    a, b = src._live(), dst._live()
+    keep = dst.capacity if keep is None else keep
+    if weights is None:
+        raise ValueError("weights are needed")
+    _whole(weights, (src.sequences, src.kv_heads, src.capacity), torch.float32, "weights", src.device)
+    _whole(weights_out, (dst.sequences, dst.kv_heads, dst.capacity), torch.float32, "weights_out", src.device)
+    _whole(kept, (src.sequences, src.kv_heads, keep), torch.int32, "kept", src.device)
+    _check(load().pxq_kv_evict(a, b, _ptr(weights), keep, recent, _ptr(weights_out), _ptr(kept), _stream_ptr(stream)))
 
 
 class _Uploaded:
