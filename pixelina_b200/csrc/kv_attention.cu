@@ -25,33 +25,8 @@
 namespace pxq {
 namespace {
 
-constexpr float kLog2E = 1.4426950408889634f;
 constexpr int AW = 8;                    // warps per CTA
 constexpr int kMinRun = 8;               // fewest blocks worth a CTA: one per warp
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// 2^e for -126 <= e <= 127
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 126; }  // |x| < 2^this
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// (a, b) = hi + lo, each half of the packed words
-__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack_half2(a - f.x, b - f.y);
-}
 
 // D += A (16 x 16, row) * B (16 x 8, column), fp16 in, fp32 out
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -77,12 +52,6 @@ __device__ __forceinline__ int kv_attn_blocks(const KvAttnCall& a, int s)
     return max(1, (q.len + kKvBlock - 1) / kKvBlock);
 }
 __device__ __forceinline__ int kv_run_length(int total, int runs) { return max(kMinRun, (total + runs - 1) / runs); }
-
-// Tokens that pair p's row sees.
-__device__ __forceinline__ int kv_limit(const KvAttnCall& a, const KvSeq& q, int i)
-{
-    return a.causal ? max(0, q.len - q.n + i + 1) : q.len;
-}
 
 // One warp's A fragments of up to PT pairs' queries: PT = 8 packs hi into
 // rows 0-7 and lo into rows 8-15 of one fragment, PT = 16 keeps two.
@@ -115,14 +84,14 @@ struct QFrag {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // |x| 2^e < 2^15; a row of zeros, or one that is not finite, stays as it is
-            const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - exponent_of(m))) : 0;
-            const float up = pow2i(e);
-            coef[u] = kLog2E / sqrtf((float)D) * pow2i(-e);
+            const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(m))) : 0;
+            const float up = kv_pow2(e);
+            coef[u] = kv_log2_inv_sqrt(D) * kv_pow2(-e);
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
                 uint32_t h0, l0, h1, l1;
-                split_half2(x[k][0] * up, x[k][1] * up, h0, l0);
-                split_half2(x[k][2] * up, x[k][3] * up, h1, l1);
+                kv_split(x[k][0] * up, x[k][1] * up, h0, l0);
+                kv_split(x[k][2] * up, x[k][3] * up, h1, l1);
                 if (PT == 8) {
                     hi[k][0] = h0, hi[k][1] = l0, hi[k][2] = h1, hi[k][3] = l1;
                 } else {
@@ -282,9 +251,9 @@ __global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ 
             // online softmax; lane (r, c) holds tokens 32 b + 8 c .. + 7 of its pairs
             const int t0 = kKvBlock * b + 8 * c;
             uint32_t ph[U][4], pl[U][4];
-            const int ev = exponent_of(sc.y);
+            const int ev = kv_exponent(sc.y);
             const int En = ev < 129 ? max(E, ev) : E;  // a NaN scale has exponent 129
-            const float up = sc.y * pow2i(15 - En);
+            const float up = sc.y * kv_pow2(15 - En);
             float corr[U];
             bool moved = En != E;
 #pragma unroll
@@ -300,22 +269,22 @@ __global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ 
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.f : mn;
-                corr[u] = ex2(m[u] - ms);
+                corr[u] = kv_ex2(m[u] - ms);
                 moved |= mn != m[u];
                 m[u] = mn;
                 float add = 0.f, y[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float p = ex2(z[u][i] - ms);
+                    const float p = kv_ex2(z[u][i] - ms);
                     add += p;
                     y[i] = t0 + i < lim[u] ? p * up : 0.f;
                 }
                 l[u] = l[u] * corr[u] + add;
 #pragma unroll
-                for (int i = 0; i < 4; i++) split_half2(y[2 * i], y[2 * i + 1], ph[u][i], pl[u][i]);
+                for (int i = 0; i < 4; i++) kv_split(y[2 * i], y[2 * i + 1], ph[u][i], pl[u][i]);
             }
             if (__any_sync(0xffffffffu, moved)) {
-                const float ef = pow2i(max(-126, E - En));
+                const float ef = kv_pow2(max(-126, E - En));
                 E = En;
                 const float c0 = corr[0] * ef, c1 = PT == 8 ? c0 : corr[U - 1] * ef;
 #pragma unroll
@@ -352,7 +321,7 @@ __global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ 
         // consumed, and each stage's phase bit is kept, so the next segment
         // starts from stage 0 again.
         float* mine = comb + warp * CW;
-        const float back = pow2i(E - 15);
+        const float back = kv_pow2(E - 15);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
@@ -387,7 +356,7 @@ __global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < AW; i++) {
                 const float* src = comb + i * CW;
-                const float f = ex2(src[p] - Ms);
+                const float f = kv_ex2(src[p] - Ms);
                 L += src[PT + p] * f;
                 O += src[2 * PT + p * D + d] * f;
             }
@@ -440,7 +409,7 @@ __global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ Attn
     float L = 0.f, O = 0.f;
     for (int i = c0; i <= c1; i++) {
         const float* src = part(i);
-        const float f = ex2(src[p] - Ms);
+        const float f = kv_ex2(src[p] - Ms);
         L += src[PT + p] * f;
         if (d < D) O += src[2 * PT + p * D + d] * f;
     }
@@ -480,7 +449,7 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
         block_scores<D, 8>(qf, rec, z);
         const float lse = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] += t0 + i < lim ? ex2(z[0][i] * (qf.coef[0] * dk) - lse) : 0.f;
+        for (int i = 0; i < 8; i++) w[i] += t0 + i < lim ? kv_ex2(z[0][i] * (qf.coef[0] * dk) - lse) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -505,6 +474,7 @@ cudaError_t by_dim(int D, F f)
 }
 
 struct AttnPlan {
+    bool prompt;
     int pt, tiles, runs;
     size_t part_bytes, lse_bytes;
 };
@@ -516,7 +486,9 @@ AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
     p.pt = pairs <= 8 ? 8 : 16;
     p.tiles = (int)((pairs + p.pt - 1) / p.pt);
     p.runs = num_sms;
-    p.part_bytes = ((size_t)p.tiles * p.runs * 2 * p.pt * (a.c.D + 2) * sizeof(float) + 255) / 256 * 256;
+    p.prompt = pairs > 16;
+    if (p.prompt) p.part_bytes = (kv_prompt_part_bytes(a, num_sms) + 255) / 256 * 256;
+    else p.part_bytes = ((size_t)p.tiles * p.runs * 2 * p.pt * (a.c.D + 2) * sizeof(float) + 255) / 256 * 256;
     p.lse_bytes = a.weights_out ? (size_t)a.rows * a.heads * sizeof(float) : 0;
     return p;
 }
@@ -549,10 +521,17 @@ cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms,
     P.part = static_cast<float*>(scratch);
     P.lse = p.lse_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.part_bytes) : nullptr;
     P.runs = p.runs;
-    *launches = a.weights_out ? 3 : 2;
+    if (p.prompt) {
+        const cudaError_t e = launch_kv_prompt(a, P.part, P.lse, num_sms, s, launches);
+        if (e != cudaSuccess || !a.weights_out) return e;
+        ++*launches;
+    } else {
+        *launches = a.weights_out ? 3 : 2;
+    }
     return by_dim(a.c.D, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        cudaError_t e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
+        cudaError_t e = cudaSuccess;
+        if (!p.prompt) e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
         if (e != cudaSuccess || !a.weights_out) return e;
         return launch_pdl(k_kv_weights<D>, dim3((unsigned)((a.c.nb + AW - 1) / AW), (unsigned)a.c.H, (unsigned)a.c.S), dim3(AW * 32), 0,
                           s, P);

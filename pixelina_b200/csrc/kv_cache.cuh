@@ -135,6 +135,37 @@ __device__ __forceinline__ bool kv_last_cta(uint32_t* ticket, uint32_t ctas, uin
 
 __device__ __forceinline__ float kv_log2_inv_sqrt(int D) { return 1.4426950408889634f / sqrtf((float)D); }
 
+__device__ __forceinline__ float kv_ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^e for -126 <= e <= 127
+__device__ __forceinline__ float kv_pow2(int e) { return __int_as_float((e + 127) << 23); }
+// |x| < 2^this; -126 for 0, 129 for what is not finite
+__device__ __forceinline__ int kv_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 126; }
+
+__device__ __forceinline__ uint32_t kv_pack(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (a, b) = hi + lo, each a pair of fp16 numbers
+__device__ __forceinline__ void kv_split(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = kv_pack(a - f.x, b - f.y);
+}
+
+// Tokens that row i of sequence q sees.
+__device__ __forceinline__ int kv_limit(const KvAttnCall& a, const KvSeq& q, int i)
+{
+    return a.causal ? max(0, q.len - q.n + i + 1) : q.len;
+}
+
 // Two fp16 numbers from two code bytes (b0, b1 or b2, b3 of w).
 __device__ __forceinline__ uint32_t kv_half2(uint32_t w, uint32_t sel)
 {

@@ -1,0 +1,571 @@
+// kv_prompt.cu -- attention of many query rows over the 8-bit key/value cache
+// on the 5th-generation tensor cores (formulas and accuracy: kv_attention.cu).
+//
+// A CTA takes 128 pairs (query row, head of the group) of one (sequence, kv
+// head) over a range of the keys, in tiles i of 128 tokens = 4 cache blocks:
+//     S_i = Qlo K^T + Qhi K^T          (fp32 in TMEM; Q hi and lo in TMEM, K the codes as fp16 in smem)
+//     P_i = exp2(S_i coef dk - m)      (hi and lo fp16, over S_i's own columns)
+//     O_i = (Plo dv) V + (Phi dv) V    (fp32 in TMEM; V the codes as fp16 in smem)
+// The scales of K enter the exponent, those of V the probabilities, so the
+// operands stay exact codes.  Warp roles (512 threads):
+//   0-3, 4-7  softmax of the even / odd key tiles, each with a max, a sum and an
+//             output of its own (joined at the end): thread = row
+//   8-11      codes -> fp16, from registers loaded a tile ahead into
+//             128-byte-swizzled smem, two buffers each for K and V
+//   12        MMA issue, in the order QK(i+1) PV(i) QK(i+2) PV(i+1): while one
+//             tile's softmax runs, the tensor core has the other parity's work
+// S_{i+2} may overwrite P_i because the products of one thread are executed
+// in the order in which it issues them.
+//
+// The tensor core cuts the accumulator's last bits at every K = 16 step, always
+// towards zero, and over a long sum that adds up: with one accumulator for a
+// whole prompt of 4096 tokens (256 steps on average) the output was off by
+// 5.6e-6 of its norm, five times what fp32 arithmetic loses.  So O_i starts at
+// zero for every tile, lo before hi (8 steps at full magnitude), and the rows'
+// sums over tiles are kept in registers, rounded to nearest.
+#include <algorithm>
+#include <type_traits>
+#include "kv_cache.cuh"
+
+namespace pxq {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kTileRows = 128;   // pairs per CTA
+constexpr int kTileKeys = 128;
+// registers per thread by role: 128 x (2 x 192 + 88 + 40) = 512 x 128, what the launch has
+constexpr uint32_t kRegsSoftmax = 192, kRegsConvert = 88, kRegsMma = 40;
+
+template <int D>
+struct PromptSmem {
+    static constexpr int K_PANEL = kTileKeys * 128;           // 128 tokens x 64 channels
+    static constexpr int K_TILE = (D + 63) / 64 * K_PANEL;
+    static constexpr int V_PANEL = D * 128;                   // D channels x 64 tokens
+    static constexpr int V_TILE = 2 * V_PANEL;
+    static constexpr int V = 2 * K_TILE;                      // after two K tiles
+    static constexpr int BYTES = V + 2 * V_TILE + 1024;       // + alignment
+    static_assert(V + 2 * V_TILE >= (D + 2) * kTileRows * 4, "the odd tiles' result fits where K and V were");
+};
+// TMEM columns
+constexpr uint32_t kColS = 0, kColO = 256, kColQ = 384;
+
+__device__ __forceinline__ uint64_t desc128(uint32_t saddr) { return smem_desc(saddr, 16, 1024, 2); }
+
+// D[tmem] (+)= A[tmem] * B[smem]^T, kind::f16
+__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 consecutive floats of a row
+__device__ __forceinline__ void row_load(const float* p, float (&x)[16], bool vec)
+{
+#pragma unroll
+    for (int c = 0; c < 16; c += 4) {
+        if (vec) {
+            const float4 v = *reinterpret_cast<const float4*>(p + c);
+            x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
+        } else {
+            x[c] = p[c], x[c + 1] = p[c + 1], x[c + 2] = p[c + 2], x[c + 3] = p[c + 3];
+        }
+    }
+}
+__device__ __forceinline__ void row_store(float* p, const float (&x)[16], bool vec)
+{
+#pragma unroll
+    for (int c = 0; c < 16; c += 4) {
+        if (vec) {
+            *reinterpret_cast<float4*>(p + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+        } else {
+            p[c] = x[c], p[c + 1] = x[c + 1], p[c + 2] = x[c + 2], p[c + 3] = x[c + 3];
+        }
+    }
+}
+
+struct PromptParams {
+    KvAttnCall a;
+    float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], O[128][D]
+    float* lse;
+    int tiles, splits;
+};
+
+__device__ __forceinline__ int prompt_tiles(const KvAttnCall& a, int s)
+{
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    if (q.n <= 0 || q.n > a.max_rows) return 0;
+    return (int)(((int64_t)q.n * (a.heads / a.c.H) + kTileRows - 1) / kTileRows);
+}
+
+// The part of a (sequence, head)'s keys that a split of one CTA takes:
+// key tiles [t0, t1) of those that the tile's last row sees.
+__device__ __forceinline__ void prompt_keys(const KvAttnCall& a, const KvSeq& q, int tile, int split, int splits, int& t0, int& t1)
+{
+    const int G = a.heads / a.c.H, pairs = q.n * G;
+    const int last = min(pairs, (tile + 1) * kTileRows) - 1;
+    const int lim = kv_limit(a, q, last / G);
+    const int n = (lim + kTileKeys - 1) / kTileKeys, per = (n + splits - 1) / splits;
+    t0 = min(n, split * per);
+    t1 = min(n, t0 + per);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant__ PromptParams P)
+{
+    using M = PromptSmem<D>;
+    constexpr uint32_t IDESC_S = idesc_f16_f32(128, kTileKeys), IDESC_O = idesc_f16_f32(128, D);
+    constexpr int J = D / 64, REC = kv_record_bytes(D);
+    extern __shared__ uint8_t dyn[];
+    __shared__ int sum[kKvMaxSequences + 1];
+    __shared__ int warp_sums[32];
+    __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_s[2], bar_p[2], bar_o_full[2], bar_o_empty, bar_fin;
+    __shared__ uint32_t tmem_slot, abort_flag;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+
+    const KvAttnCall& a = P.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.x % a.c.H, gt = P.tiles - 1 - blockIdx.x / a.c.H, split = blockIdx.y, G = a.heads / a.c.H;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar_k_full[i], 128);
+            mbar_init(&bar_k_empty[i], 1);
+            mbar_init(&bar_v_full[i], 128);
+            mbar_init(&bar_v_empty[i], 1);
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[i], 128);
+            mbar_init(&bar_o_full[i], 1);
+        }
+        mbar_init(&bar_o_empty, 128);
+        mbar_init(&bar_fin, 1);
+        fence_mbar_init();
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
+        const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
+        return prompt_tiles(a, s);
+    });
+    if (gt >= sum[a.c.S]) return;
+    const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const int pairs = q.n * G;
+    int t0, t1;
+    prompt_keys(a, q, tile, split, P.splits, t0, t1);
+    const int n = t1 - t0;
+    const int64_t sh = (int64_t)s * a.c.H + h;
+    const uint8_t* recs = a.c.codes + sh * a.c.nb * (int64_t)REC;
+    const float2* scales = a.c.scales + sh * a.c.nb;
+
+    if (warp == 12) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int X = warp / 4, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    int lim = 0, head = 0;
+    int64_t out_row = 0;
+    float coef = 0.f;
+    bool live = false;
+    if (warp < 8) {  // the rows' queries: scaled to below 2^15, split, stored by the first four warps
+        const int p = tile * kTileRows + row;
+        live = p < pairs;
+        out_row = q.row0 + (live ? p / G : 0);
+        head = h * G + (live ? p % G : 0);
+        lim = live ? kv_limit(a, q, p / G) : 0;
+        const float* src = a.q + out_row * a.ldq + (int64_t)head * D;
+        const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
+        float m = 0.f;
+#pragma unroll 2
+        for (int d = 0; d < D; d += 16) {
+            float x[16];
+            if (live) row_load(src + d, x, vec);
+#pragma unroll
+            for (int i = 0; i < 16; i++) m = live ? fmaxf(m, fabsf(x[i])) : 0.f;
+        }
+        const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(m))) : 0;
+        const float up = kv_pow2(e);
+        coef = kv_log2_inv_sqrt(D) * kv_pow2(-e);
+        if (X == 0) {
+#pragma unroll 2
+            for (int d = 0; d < D; d += 16) {
+                float x[16];
+                uint32_t hi[8], lo[8];
+                if (live) row_load(src + d, x, vec);
+#pragma unroll
+                for (int i = 0; i < 8; i++) kv_split(live ? x[2 * i] * up : 0.f, live ? x[2 * i + 1] * up : 0.f, hi[i], lo[i]);
+                tmem_st8(tmem + lanes + kColQ + d / 2, hi);
+                tmem_st8(tmem + lanes + kColQ + D / 2 + d / 2, lo);
+            }
+            tmem_st_wait();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t* status = a.status;
+
+    if (warp < 8) {
+        regs_inc<kRegsSoftmax>();
+        const uint32_t ts = tmem + lanes + kColS + X * 128, to = tmem + lanes + kColO;
+        float m = -INFINITY, l = 0.f, o[D];
+        int E = -100;  // o is in units of 2^(E - 15)
+        bool ok = true;
+#pragma unroll
+        for (int d = 0; d < D; d++) o[d] = 0.f;
+        for (int i = X; i < n; i += 2) {
+            const int key0 = (t0 + i) * kTileKeys;
+            float dk[4], dv[4];
+            int En = E;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int b = key0 / kKvBlock + j;
+                const bool any = b * kKvBlock < q.len;  // blocks past the end hold anything
+                const float2 sc = any ? scales[b] : make_float2(0.f, 0.f);
+                dk[j] = coef * sc.x;
+                dv[j] = sc.y;
+                const int x = kv_exponent(sc.y);
+                if (x < 129) En = max(En, x);  // 129: NaN
+            }
+            if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
+            float mn = m;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t r[32];
+                tmem_ld32(ts + 32 * j, r);
+                tmem_ld_wait_dep(r);
+                float mx = -INFINITY;
+                if (full) {
+#pragma unroll
+                    for (int c = 0; c < 32; c++) mx = fmaxf(mx, __uint_as_float(r[c]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; c++)
+                        if (key0 + 32 * j + c < lim) mx = fmaxf(mx, __uint_as_float(r[c]));
+                }
+                if (mx != -INFINITY) mn = fmaxf(mn, mx * dk[j]);
+            }
+            const float ms = mn == -INFINITY ? 0.f : mn;
+            const float f = kv_ex2(m - ms);
+            const float g = f * kv_pow2(max(-126, E - En));
+            m = mn;
+            E = En;
+            const float unit = kv_pow2(15 - En);
+            float add0 = 0.f, add1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                uint32_t r[16], hi[8], lo[8];
+                tmem_ld16(ts + 16 * j, r);
+                tmem_ld_wait_dep(r);
+                const float k = dk[j / 2], y = dv[j / 2] * unit;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    float p0 = kv_ex2(__fmaf_rn(__uint_as_float(r[2 * c]), k, -ms));
+                    float p1 = kv_ex2(__fmaf_rn(__uint_as_float(r[2 * c + 1]), k, -ms));
+                    float y0 = p0 * y, y1 = p1 * y;
+                    if (!full) {
+                        const int t = key0 + 16 * j + 2 * c;
+                        if (t >= lim) p0 = y0 = 0.f;
+                        if (t + 1 >= lim) p1 = y1 = 0.f;
+                    }
+                    add0 += p0;
+                    add1 += p1;
+                    kv_split(y0, y1, hi[c], lo[c]);
+                }
+                tmem_st8(ts + 16 * j, hi);
+                tmem_st8(ts + 16 * j + 8, lo);
+            }
+            l = l * f + (add0 + add1);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&bar_p[X]);
+            if (!mbar_wait(&bar_o_full[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int d = 0; d < D; d += 16) {
+                uint32_t r[16];
+                tmem_ld16(to + d, r);
+                tmem_ld_wait_dep(r);
+#pragma unroll
+                for (int c = 0; c < 16; c++) o[d + c] = __fmaf_rn(o[d + c], g, __uint_as_float(r[c]));
+            }
+            tc_fence_before();
+            mbar_arrive(&bar_o_empty);
+        }
+        // the odd tiles' sums go through smem (free once every product is done) to the even tiles' threads
+        if (ok && n > 0) ok = mbar_wait(&bar_fin, 0, &abort_flag, status, kDevTimeoutTmemFull);
+        float* other = reinterpret_cast<float*>(smem) + row;  // [m, l, O[D]][128 rows]
+        const float back = kv_pow2(E - 15);
+        if (X == 1) {
+            other[0] = m;
+            other[kTileRows] = l;
+#pragma unroll
+            for (int d = 0; d < D; d++) other[(2 + d) * kTileRows] = o[d] * back;
+        }
+        named_bar_sync(1, 256);
+        if (X == 0 && ok && live) {
+            const float m1 = other[0], l1 = other[kTileRows], mn = fmaxf(m, m1), ms = mn == -INFINITY ? 0.f : mn;
+            const float f0 = kv_ex2(m - ms), f1 = kv_ex2(m1 - ms);
+            l = l * f0 + l1 * f1;
+            const bool none = mn == -INFINITY && l == 0.f;  // on the max too: a NaN sum stays NaN
+            float* part = P.part + (((int64_t)split * P.tiles + gt) * a.c.H + h) * kTileRows * (D + 2);
+            float* dst = a.out + out_row * a.ldo + (int64_t)head * D;
+            bool vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0;
+            float scale = none ? 0.f : __fdiv_rn(1.f, l);
+            if (P.splits > 1) {
+                part[row] = mn;
+                part[kTileRows + row] = l;
+                dst = part + 2 * kTileRows + (int64_t)row * D;
+                vec = true;
+                scale = 1.f;
+            } else if (P.lse) {
+                P.lse[out_row * a.heads + head] = none ? INFINITY : mn + log2f(l);
+            }
+            const float c0 = f0 * back;
+#pragma unroll
+            for (int d = 0; d < D; d += 16) {
+                float x[16];
+#pragma unroll
+                for (int c = 0; c < 16; c++) x[c] = (o[d + c] * c0 + other[(2 + d + c) * kTileRows] * f1) * scale;
+                row_store(dst + d, x, vec);
+            }
+        }
+    } else if (warp < 12) {
+        regs_dec<kRegsConvert>();
+        const int cw = warp - 8, qn = lane / 4, qc = lane % 4;
+        uint4 kr[4 * J + (D % 64 ? 1 : 0)], vr[D / 16];
+        const uint32_t sb = smem_u32(smem);
+        // Blocks of key tile i: for K this warp's own; for V lanes of even and odd qn take the two blocks of the warp's
+        // half tile, so that eight lanes' 16-byte stores fall in different banks.  Past the cache's end: its last
+        // block (masked).
+        const int bv = cw / 2 * 2 + ((qn ^ cw) & 1);
+        auto record = [&](int i, int b) { return recs + (int64_t)min((t0 + i) * (kTileKeys / kKvBlock) + b, a.c.nb - 1) * REC + lane * 16; };
+        auto load_k = [&](int i) {
+            const uint8_t* r = record(i, cw);
+#pragma unroll
+            for (int u = 0; u < 4 * J + (D % 64 ? 1 : 0); u++) kr[u] = *reinterpret_cast<const uint4*>(r + u * 512);
+        };
+        auto load_v = [&](int i) {
+            const uint8_t* r = record(i, bv) + 32 * D;
+#pragma unroll
+            for (int u = 0; u < D / 16; u++) vr[u] = *reinterpret_cast<const uint4*>(r + u * 512);
+        };
+        auto st128 = [](uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+        };
+        if (n > 0) {
+            load_k(0);
+            load_v(0);
+        }
+        for (int i = 0; i < n; i++) {
+            const int B = i & 1;
+            const uint32_t ph = ((i >> 1) - 1) & 1, kb = sb + B * M::K_TILE, vb = sb + M::V + B * M::V_TILE;
+            if (i > 1 && !mbar_wait(&bar_k_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
+#pragma unroll
+            for (int nt = 0; nt < 4; nt++) {
+                const int t = 32 * cw + 8 * (qn / 2) + 2 * nt + qn % 2;  // row of the key tile
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+                    const uint4 w = kr[nt * J + j];
+                    const uint32_t at = kb + j * M::K_PANEL + t * 128;
+                    st128(at + (((2 * qc) ^ (t & 7)) << 4), kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
+                    st128(at + (((2 * qc + 1) ^ (t & 7)) << 4), kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
+                }
+                if (D % 64) {
+                    const uint4 w = kr[4 * J];
+                    const uint32_t x = nt == 0 ? w.x : nt == 1 ? w.y : nt == 2 ? w.z : w.w;
+                    const uint32_t at = kb + J * M::K_PANEL + t * 128 + (((qc / 2) ^ (t & 7)) << 4) + qc % 2 * 8;
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(kv_half2_lo(x)), "r"(kv_half2_hi(x)) : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bar_k_full[B]);
+            if (i + 1 < n) load_k(i + 1);
+            if (i > 1 && !mbar_wait(&bar_v_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
+#pragma unroll
+            for (int np = 0; np < D / 16; np++) {
+                const uint4 w = vr[np];
+#pragma unroll
+                for (int f = 0; f < 2; f++) {
+                    const int ch = 8 * (2 * np + f) + qn;
+                    const uint32_t x = f ? w.z : w.x, y = f ? w.w : w.y;
+                    st128(vb + cw / 2 * M::V_PANEL + ch * 128 + (((4 * (bv & 1) + qc) ^ qn) << 4), kv_half2_lo(x), kv_half2_hi(x),
+                          kv_half2_lo(y), kv_half2_hi(y));
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bar_v_full[B]);
+            if (i + 1 < n) load_v(i + 1);
+        }
+    } else {
+        regs_dec<kRegsMma>();
+        if (warp == 12 && lane == 0 && n > 0) {
+            const uint32_t sb = smem_u32(smem);
+            auto qk = [&](int i) {
+                const int B = i & 1;
+                if (!mbar_wait(&bar_k_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int lo = 1; lo >= 0; lo--)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)
+                        mma_f16_ta(tmem + kColS + B * 128, tmem + kColQ + lo * (D / 2) + k * 8,
+                                   desc128(sb + B * M::K_TILE + k / 4 * M::K_PANEL + k % 4 * 32), IDESC_S, !lo || k);
+                mma_commit(&bar_s[B]);
+                mma_commit(&bar_k_empty[B]);
+                return true;
+            };
+            auto pv = [&](int i) {
+                const int B = i & 1;
+                if (!mbar_wait(&bar_v_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
+                if (i > 0 && !mbar_wait(&bar_o_empty, (i - 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
+                if (!mbar_wait(&bar_p[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int lo = 1; lo >= 0; lo--)
+#pragma unroll
+                    for (int k = 0; k < kTileKeys / 16; k++)
+                        mma_f16_ta(tmem + kColO, tmem + kColS + B * 128 + k * 16 + lo * 8,
+                                   desc128(sb + M::V + B * M::V_TILE + k / 4 * M::V_PANEL + k % 4 * 32), IDESC_O, !lo || k);
+                mma_commit(&bar_o_full[B]);
+                mma_commit(&bar_v_empty[B]);
+                return true;
+            };
+            bool ok = qk(0) && (n < 2 || qk(1));
+            for (int i = 0; ok && i < n; i++) ok = pv(i) && (i + 2 >= n || qk(i + 2));
+            // nothing of this CTA may still run when its TMEM is freed
+            mma_commit(&bar_fin);
+            for (int i = 0; i < 2000 && !mbar_try_wait(&bar_fin, 0); i++) {}
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the key splits: one warp per pair of a (tile, head).
+template <int D>
+__global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptParams P)
+{
+    __shared__ int sum[kKvMaxSequences + 1];
+    __shared__ int warp_sums[32];
+    const KvAttnCall& a = P.a;
+    griddep_wait();
+    griddep_launch_dependents();
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles(a, s); });
+    const int gt = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, G = a.heads / a.c.H;
+    if (gt >= sum[a.c.S]) return;
+    const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const int pr = blockIdx.z * 8 + (threadIdx.x >> 5), p = tile * kTileRows + pr;
+    if (p >= q.n * G) return;
+    int t0, t1;
+    prompt_keys(a, q, tile, 0, P.splits, t0, t1);
+    const int per = max(1, t1 - t0);
+    prompt_keys(a, q, tile, 0, 1, t0, t1);
+    const int used = (t1 + per - 1) / per;  // splits that had keys
+    const int64_t step = (int64_t)P.tiles * a.c.H * kTileRows * (D + 2);
+    const float* part = P.part + ((int64_t)gt * a.c.H + h) * kTileRows * (D + 2);
+    float m = -INFINITY;
+    for (int i = 0; i < used; i++) m = fmaxf(m, part[i * step + pr]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[(D + 31) / 32];
+#pragma unroll
+    for (int u = 0; u < (D + 31) / 32; u++) o[u] = 0.f;
+    for (int i = 0; i < used; i++) {
+        const float* src = part + i * step;
+        const float f = kv_ex2(src[pr] - ms);
+        l += src[kTileRows + pr] * f;
+#pragma unroll
+        for (int u = 0; u < (D + 31) / 32; u++)
+            if (32 * u + lane < D) o[u] += src[2 * kTileRows + (int64_t)pr * D + 32 * u + lane] * f;
+    }
+    const bool none = m == -INFINITY && l == 0.f;
+    const int64_t row = q.row0 + p / G;
+    const int head = h * G + p % G;
+    const float f = __fdiv_rn(1.f, l);
+#pragma unroll
+    for (int u = 0; u < (D + 31) / 32; u++)
+        if (32 * u + lane < D) a.out[row * a.ldo + (int64_t)head * D + 32 * u + lane] = none ? 0.f : o[u] * f;
+    if (P.lse && lane == 0) P.lse[row * a.heads + head] = none ? INFINITY : m + log2f(l);
+}
+
+struct PromptPlan {
+    int tiles, splits;
+    size_t part_bytes;
+};
+
+PromptPlan plan_prompt(const KvAttnCall& a, int num_sms)
+{
+    PromptPlan p{};
+    const int64_t G = a.heads / a.c.H;
+    // a sequence's n rows make at most n G / 128 + 1 tiles
+    const int64_t most = std::min<int64_t>(a.c.S * ((a.max_rows * G + kTileRows - 1) / kTileRows), a.rows * G / kTileRows + a.c.S);
+    p.tiles = (int)most;
+    const int64_t key_tiles = (a.c.cap + kTileKeys - 1) / kTileKeys;
+    p.splits = (int)std::max<int64_t>(1, std::min(key_tiles, num_sms / (most * a.c.H)));
+    p.part_bytes = p.splits > 1 ? (size_t)p.splits * p.tiles * a.c.H * kTileRows * (a.c.D + 2) * sizeof(float) : 0;
+    return p;
+}
+
+template <int D>
+cudaError_t launch_d(const PromptParams& P, cudaStream_t s)
+{
+    constexpr int smem = PromptSmem<D>::BYTES;
+    cudaError_t e = cudaFuncSetAttribute(k_kv_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_kv_prompt<D>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
+    if (e != cudaSuccess || P.splits == 1) return e;
+    const int64_t pairs = std::min<int64_t>(kTileRows, P.a.max_rows * (P.a.heads / P.a.c.H));
+    return launch_pdl(k_kv_join<D>, dim3((unsigned)P.tiles, (unsigned)P.a.c.H, (unsigned)((pairs + 7) / 8)), dim3(256), 0, s, P);
+}
+
+}  // namespace
+
+size_t kv_prompt_part_bytes(const KvAttnCall& a, int num_sms) { return plan_prompt(a, num_sms).part_bytes; }
+
+cudaError_t launch_kv_prompt(const KvAttnCall& a, float* part, float* lse, int num_sms, cudaStream_t s, int* launches)
+{
+    const PromptPlan p = plan_prompt(a, num_sms);
+    PromptParams P{};
+    P.a = a;
+    P.part = part;
+    P.lse = lse;
+    P.tiles = p.tiles;
+    P.splits = p.splits;
+    *launches = p.splits > 1 ? 2 : 1;
+    switch (a.c.D) {
+    case 64: return launch_d<64>(P, s);
+    case 80: return launch_d<80>(P, s);
+    case 128: return launch_d<128>(P, s);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace pxq

@@ -216,6 +216,9 @@ struct KvAttnCall {
     float* weights_out;      // null: no weights wanted
     uint32_t* status;
 };
+// kv_prompt.cu: more than 16 pairs (query row, head of a group); lse: null or [rows][heads]
+size_t kv_prompt_part_bytes(const KvAttnCall& a, int num_sms);
+cudaError_t launch_kv_prompt(const KvAttnCall& a, float* part, float* lse, int num_sms, cudaStream_t s, int* launches);
 size_t kv_attention_scratch_bytes(const KvAttnCall& a, int num_sms);
 // *launches: kernels launched
 cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms, cudaStream_t s, int* launches);
