@@ -33,8 +33,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kTileRows = 128;   // pairs per CTA
 constexpr int kTileKeys = 128;
-// registers per thread by role: 128 x (2 x 192 + 88 + 40) = 512 x 128, what the launch has
-constexpr uint32_t kRegsSoftmax = 192, kRegsConvert = 88, kRegsMma = 40;
+// registers per thread by role: 128 x (2 x 200 + 80 + 32) = 512 x 128, what the launch has
+constexpr uint32_t kRegsSoftmax = 200, kRegsConvert = 80, kRegsMma = 32;
 
 template <int D>
 struct PromptSmem {
@@ -229,73 +229,87 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         bool ok = true;
 #pragma unroll
         for (int d = 0; d < D; d++) o[d] = 0.f;
+        float2 next[4];
+        auto fetch = [&](int i) {  // scales of key tile i; blocks past the end hold anything
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int b = (t0 + i) * (kTileKeys / kKvBlock) + j;
+                next[j] = i < n && b * kKvBlock < q.len ? scales[b] : make_float2(0.f, 0.f);
+            }
+        };
+        fetch(X);
         for (int i = X; i < n; i += 2) {
             const int key0 = (t0 + i) * kTileKeys;
             float dk[4], dv[4];
             int En = E;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int b = key0 / kKvBlock + j;
-                const bool any = b * kKvBlock < q.len;  // blocks past the end hold anything
-                const float2 sc = any ? scales[b] : make_float2(0.f, 0.f);
-                dk[j] = coef * sc.x;
-                dv[j] = sc.y;
-                const int x = kv_exponent(sc.y);
+                dk[j] = coef * next[j].x;
+                dv[j] = next[j].y;
+                const int x = kv_exponent(dv[j]);
                 if (x < 129) En = max(En, x);  // 129: NaN
             }
+            fetch(i + 2);
             if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
-            float mn = m;
+            const float mo = m;
+            // TMEM loads run one chunk of 16 tokens ahead of their use
+            auto maxima = [&](auto masked) {
+                uint32_t r[2][16];
+                tmem_ld16(ts, r[0]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t r[32];
-                tmem_ld32(ts + 32 * j, r);
-                tmem_ld_wait_dep(r);
-                float mx = -INFINITY;
-                if (full) {
+                for (int j = 0; j < 8; j++) {
+                    tmem_ld_wait_dep(r[j & 1]);
+                    if (j < 7) tmem_ld16(ts + 16 * (j + 1), r[(j + 1) & 1]);
+                    float mx = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 32; c++) mx = fmaxf(mx, __uint_as_float(r[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; c++)
-                        if (key0 + 32 * j + c < lim) mx = fmaxf(mx, __uint_as_float(r[c]));
+                    for (int c = 0; c < 16; c++)
+                        if (!decltype(masked)::value || key0 + 16 * j + c < lim) mx = fmaxf(mx, __uint_as_float(r[j & 1][c]));
+                    if (!decltype(masked)::value || mx != -INFINITY) m = fmaxf(m, mx * dk[j / 2]);
                 }
-                if (mx != -INFINITY) mn = fmaxf(mn, mx * dk[j]);
-            }
-            const float ms = mn == -INFINITY ? 0.f : mn;
-            const float f = kv_ex2(m - ms);
+            };
+            if (full) maxima(std::false_type{});
+            else maxima(std::true_type{});
+            const float ms = m == -INFINITY ? 0.f : m;
+            const float f = kv_ex2(mo - ms);
             const float g = f * kv_pow2(max(-126, E - En));
-            m = mn;
-            E = En;
             const float unit = kv_pow2(15 - En);
+            E = En;
             float add0 = 0.f, add1 = 0.f;
+            auto weigh = [&](auto masked) {
+                uint32_t r[2][16];
+                tmem_ld16(ts, r[0]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                uint32_t r[16], hi[8], lo[8];
-                tmem_ld16(ts + 16 * j, r);
-                tmem_ld_wait_dep(r);
-                const float k = dk[j / 2], y = dv[j / 2] * unit;
+                for (int j = 0; j < 8; j++) {
+                    uint32_t hi[8], lo[8];
+                    tmem_ld_wait_dep(r[j & 1]);
+                    if (j < 7) tmem_ld16(ts + 16 * (j + 1), r[(j + 1) & 1]);
+                    const float k = dk[j / 2], y = dv[j / 2] * unit;
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    float p0 = kv_ex2(__fmaf_rn(__uint_as_float(r[2 * c]), k, -ms));
-                    float p1 = kv_ex2(__fmaf_rn(__uint_as_float(r[2 * c + 1]), k, -ms));
-                    float y0 = p0 * y, y1 = p1 * y;
-                    if (!full) {
-                        const int t = key0 + 16 * j + 2 * c;
-                        if (t >= lim) p0 = y0 = 0.f;
-                        if (t + 1 >= lim) p1 = y1 = 0.f;
+                    for (int c = 0; c < 8; c++) {
+                        float p0 = -ms, p1 = -ms, y0, y1;
+                        ffma2(p0, p1, __uint_as_float(r[j & 1][2 * c]), __uint_as_float(r[j & 1][2 * c + 1]), k, k);
+                        p0 = kv_ex2(p0);
+                        p1 = kv_ex2(p1);
+                        fmul2(y0, y1, p0, p1, y, y);
+                        if (decltype(masked)::value) {
+                            const int t = key0 + 16 * j + 2 * c;
+                            if (t >= lim) p0 = y0 = 0.f;
+                            if (t + 1 >= lim) p1 = y1 = 0.f;
+                        }
+                        ffma2(add0, add1, p0, p1, 1.f, 1.f);
+                        kv_split(y0, y1, hi[c], lo[c]);
                     }
-                    add0 += p0;
-                    add1 += p1;
-                    kv_split(y0, y1, hi[c], lo[c]);
+                    tmem_st8(ts + 16 * j, hi);
+                    tmem_st8(ts + 16 * j + 8, lo);
                 }
-                tmem_st8(ts + 16 * j, hi);
-                tmem_st8(ts + 16 * j + 8, lo);
-            }
+            };
+            if (full) weigh(std::false_type{});
+            else weigh(std::true_type{});
             l = l * f + (add0 + add1);
             tmem_st_wait();
             tc_fence_before();
@@ -305,13 +319,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 break;
             }
             tc_fence_after();
+            {
+                uint32_t r[2][16];
+                tmem_ld16(to, r[0]);
 #pragma unroll
-            for (int d = 0; d < D; d += 16) {
-                uint32_t r[16];
-                tmem_ld16(to + d, r);
-                tmem_ld_wait_dep(r);
+                for (int d = 0; d < D; d += 16) {
+                    tmem_ld_wait_dep(r[d / 16 & 1]);
+                    if (d + 16 < D) tmem_ld16(to + d + 16, r[(d / 16 + 1) & 1]);
 #pragma unroll
-                for (int c = 0; c < 16; c++) o[d + c] = __fmaf_rn(o[d + c], g, __uint_as_float(r[c]));
+                    for (int c = 0; c < 16; c++) o[d + c] = __fmaf_rn(o[d + c], g, __uint_as_float(r[d / 16 & 1][c]));
+                }
             }
             tc_fence_before();
             mbar_arrive(&bar_o_empty);
