@@ -7,13 +7,15 @@
 //     P_i = exp2(S_i coef dk - m)      (hi and lo fp16, over S_i's own columns)
 //     O_i = (Plo dv) V + (Phi dv) V    (fp32 in TMEM; V the codes as fp16 in smem)
 // The scales of K enter the exponent, those of V the probabilities, so the
-// operands stay exact codes.  Warp roles (512 threads):
-//   0-3, 4-7  softmax of the even / odd key tiles, each with a max, a sum and an
-//             output of its own (joined at the end): thread = row
-//   8-11      codes -> fp16, from registers loaded a tile ahead into
-//             128-byte-swizzled smem, two buffers each for K and V
-//   12        MMA issue, in the order QK(i+1) PV(i) QK(i+2) PV(i+1): while one
-//             tile's softmax runs, the tensor core has the other parity's work
+// operands stay exact codes.  Warp roles (640 threads):
+//   0-3, 4-7  softmax of the even / odd key tiles, thread = row; the running max
+//             goes from one to the other through smem
+//   8-11      sums of the O_i, in registers, thread = row; the output
+//   12-15     codes (bulk copies, two tiles ahead) -> fp16 in 128-byte-swizzled
+//             smem, two buffers each for K and V
+//   16        MMA issue, in the order QK(i+1) PV(i) QK(i+2) PV(i+1): while one
+//             tile's softmax runs, the tensor core has the other parity's work;
+//             PV(i) starts when the first half of P_i is there
 // S_{i+2} may overwrite P_i because the products of one thread are executed
 // in the order in which it issues them.
 //
@@ -21,8 +23,8 @@
 // towards zero, and over a long sum that adds up: with one accumulator for a
 // whole prompt of 4096 tokens (256 steps on average) the output was off by
 // 5.6e-6 of its norm, five times what fp32 arithmetic loses.  So O_i starts at
-// zero for every tile, lo before hi (8 steps at full magnitude), and the rows'
-// sums over tiles are kept in registers, rounded to nearest.
+// zero for every tile, and the rows' sums over tiles are kept in registers,
+// rounded to nearest.
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"
@@ -30,11 +32,11 @@
 namespace pxq {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kTileRows = 128;   // pairs per CTA
 constexpr int kTileKeys = 128;
-// registers per thread by role: 128 x (2 x 200 + 80 + 32) = 512 x 128, what the launch has
-constexpr uint32_t kRegsSoftmax = 200, kRegsConvert = 80, kRegsMma = 32;
+// registers per thread by role: 128 x (2 x 104 + 168 + 80 + 24) = 640 x 96, what the launch has
+constexpr uint32_t kRegsSoftmax = 104, kRegsSum = 168, kRegsConvert = 80, kRegsMma = 24;
 
 template <int D>
 struct PromptSmem {
@@ -43,8 +45,9 @@ struct PromptSmem {
     static constexpr int V_PANEL = D * 128;                   // D channels x 64 tokens
     static constexpr int V_TILE = 2 * V_PANEL;
     static constexpr int V = 2 * K_TILE;                      // after two K tiles
-    static constexpr int BYTES = V + 2 * V_TILE + 1024;       // + alignment
-    static_assert(V + 2 * V_TILE >= (D + 2) * kTileRows * 4, "the odd tiles' result fits where K and V were");
+    static constexpr int RAW_TILE = 4 * kv_record_bytes(D);   // the codes of a key tile
+    static constexpr int RAW = V + 2 * V_TILE;
+    static constexpr int BYTES = RAW + 2 * RAW_TILE + 1024;   // + alignment
 };
 // TMEM columns
 constexpr uint32_t kColS = 0, kColO = 256, kColQ = 384;
@@ -129,7 +132,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     extern __shared__ uint8_t dyn[];
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
-    __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_s[2], bar_p[2], bar_o_full[2], bar_o_empty, bar_fin;
+    __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_s[2], bar_m[2], bar_p[2][2], bar_o_full[2],
+        bar_o_empty, bar_fin;
+    __shared__ float row_max[2][kTileRows], row_sum[2][kTileRows], row_gain[4][kTileRows];  // by tile's parity; gain by tile % 4
+    __shared__ int unit_exp[2];
     __shared__ uint32_t tmem_slot, abort_flag;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
 
@@ -143,8 +149,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_init(&bar_k_empty[i], 1);
             mbar_init(&bar_v_full[i], 128);
             mbar_init(&bar_v_empty[i], 1);
+            mbar_init(&bar_raw[i], 4);
             mbar_init(&bar_s[i], 1);
-            mbar_init(&bar_p[i], 128);
+            mbar_init(&bar_m[i], 128);
+            mbar_init(&bar_p[i][0], 128);
+            mbar_init(&bar_p[i][1], 128);
             mbar_init(&bar_o_full[i], 1);
         }
         mbar_init(&bar_o_empty, 128);
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     const uint8_t* recs = a.c.codes + sh * a.c.nb * (int64_t)REC;
     const float2* scales = a.c.scales + sh * a.c.nb;
 
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
     }
@@ -183,12 +192,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     int64_t out_row = 0;
     float coef = 0.f;
     bool live = false;
-    if (warp < 8) {  // the rows' queries: scaled to below 2^15, split, stored by the first four warps
+    if (warp < 12) {
         const int p = tile * kTileRows + row;
         live = p < pairs;
         out_row = q.row0 + (live ? p / G : 0);
         head = h * G + (live ? p % G : 0);
         lim = live ? kv_limit(a, q, p / G) : 0;
+    }
+    if (warp < 8) {  // the rows' queries: scaled to below 2^15, split, stored by the first four warps
         const float* src = a.q + out_row * a.ldq + (int64_t)head * D;
         const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
         float m = 0.f;
@@ -223,131 +234,145 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
 
     if (warp < 8) {
         regs_inc<kRegsSoftmax>();
-        const uint32_t ts = tmem + lanes + kColS + X * 128, to = tmem + lanes + kColO;
-        float m = -INFINITY, l = 0.f, o[D];
-        int E = -100;  // o is in units of 2^(E - 15)
-        bool ok = true;
-#pragma unroll
-        for (int d = 0; d < D; d++) o[d] = 0.f;
-        float2 next[4];
-        auto fetch = [&](int i) {  // scales of key tile i; blocks past the end hold anything
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int b = (t0 + i) * (kTileKeys / kKvBlock) + j;
-                next[j] = i < n && b * kKvBlock < q.len ? scales[b] : make_float2(0.f, 0.f);
-            }
+        const uint32_t ts = tmem + lanes + kColS + X * 128;
+        float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
+        int E = -100;                  // P_i holds p (dv / 2^(E - 15))
+        // lane j < 4: the scales of key tile i's block j; blocks past the end hold anything
+        auto fetch = [&](int i) {
+            const int b = (t0 + i) * (kTileKeys / kKvBlock) + lane;
+            return lane < 4 && i < n && b * kKvBlock < q.len ? scales[b] : make_float2(0.f, 0.f);
         };
-        fetch(X);
+        float2 next = fetch(X);
         for (int i = X; i < n; i += 2) {
             const int key0 = (t0 + i) * kTileKeys;
-            float dk[4], dv[4];
-            int En = E;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                dk[j] = coef * next[j].x;
-                dv[j] = next[j].y;
-                const int x = kv_exponent(dv[j]);
-                if (x < 129) En = max(En, x);  // 129: NaN
-            }
-            fetch(i + 2);
-            if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
-                ok = false;
-                break;
-            }
+            const float2 sc = next;
+            next = fetch(i + 2);
+            const int x = kv_exponent(sc.y);
+            const int ev = __reduce_max_sync(0xffffffffu, x < 129 ? x : -100);  // 129: NaN
+            if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) break;
             tc_fence_after();
             const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
-            const float mo = m;
+            float mt = -INFINITY;
             // TMEM loads run one chunk of 16 tokens ahead of their use
             auto maxima = [&](auto masked) {
                 uint32_t r[2][16];
                 tmem_ld16(ts, r[0]);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    tmem_ld_wait_dep(r[j & 1]);
-                    if (j < 7) tmem_ld16(ts + 16 * (j + 1), r[(j + 1) & 1]);
+#pragma unroll 1
+                for (int j = 0; j < 4; j++) {
                     float mx = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 16; c++)
-                        if (!decltype(masked)::value || key0 + 16 * j + c < lim) mx = fmaxf(mx, __uint_as_float(r[j & 1][c]));
-                    if (!decltype(masked)::value || mx != -INFINITY) m = fmaxf(m, mx * dk[j / 2]);
+                    for (int u = 0; u < 2; u++) {
+                        tmem_ld_wait_dep(r[u]);
+                        tmem_ld16(ts + (32 * j + 16 * u + 16) % kTileKeys, r[u ^ 1]);
+#pragma unroll
+                        for (int c = 0; c < 16; c++)
+                            if (!decltype(masked)::value || key0 + 32 * j + 16 * u + c < lim) mx = fmaxf(mx, __uint_as_float(r[u][c]));
+                    }
+                    const float k = coef * __shfl_sync(0xffffffffu, sc.x, j);
+                    if (!decltype(masked)::value || mx != -INFINITY) mt = fmaxf(mt, mx * k);
                 }
+                tmem_ld_wait_dep(r[0]);
             };
             if (full) maxima(std::false_type{});
             else maxima(std::true_type{});
-            const float ms = m == -INFINITY ? 0.f : m;
-            const float f = kv_ex2(mo - ms);
-            const float g = f * kv_pow2(max(-126, E - En));
-            const float unit = kv_pow2(15 - En);
-            E = En;
+            // the max and the unit of the tiles before, from the other parity
+            float mp = -INFINITY;
+            int Ep = -100;
+            if (i > 0) {
+                if (!mbar_wait(&bar_m[X ^ 1], ((i - 1) >> 1) & 1, &abort_flag, status, kDevTimeoutScaleFull)) break;
+                mp = row_max[X ^ 1][row];
+                Ep = unit_exp[X ^ 1];
+            }
+            const float mn = fmaxf(mp, mt), ms = mn == -INFINITY ? 0.f : mn;
+            E = max(Ep, ev);
+            row_max[X][row] = mn;
+            if (row == 0) unit_exp[X] = E;
+            mbar_arrive(&bar_m[X]);
+            row_gain[i & 3][row] = kv_ex2(mp - ms) * kv_pow2(max(-126, Ep - E));
+            l *= kv_ex2(m - ms);
+            m = mn;
+            const float unit = kv_pow2(15 - E);
             float add0 = 0.f, add1 = 0.f;
             auto weigh = [&](auto masked) {
                 uint32_t r[2][16];
                 tmem_ld16(ts, r[0]);
+#pragma unroll 1
+                for (int j = 0; j < 4; j++) {
+                    const float k = coef * __shfl_sync(0xffffffffu, sc.x, j), y = unit * __shfl_sync(0xffffffffu, sc.y, j);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    uint32_t hi[8], lo[8];
-                    tmem_ld_wait_dep(r[j & 1]);
-                    if (j < 7) tmem_ld16(ts + 16 * (j + 1), r[(j + 1) & 1]);
-                    const float k = dk[j / 2], y = dv[j / 2] * unit;
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t hi[8], lo[8];
+                        tmem_ld_wait_dep(r[u]);
+                        tmem_ld16(ts + (32 * j + 16 * u + 16) % kTileKeys, r[u ^ 1]);
 #pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        float p0 = -ms, p1 = -ms, y0, y1;
-                        ffma2(p0, p1, __uint_as_float(r[j & 1][2 * c]), __uint_as_float(r[j & 1][2 * c + 1]), k, k);
-                        p0 = kv_ex2(p0);
-                        p1 = kv_ex2(p1);
-                        fmul2(y0, y1, p0, p1, y, y);
-                        if (decltype(masked)::value) {
-                            const int t = key0 + 16 * j + 2 * c;
-                            if (t >= lim) p0 = y0 = 0.f;
-                            if (t + 1 >= lim) p1 = y1 = 0.f;
+                        for (int c = 0; c < 8; c++) {
+                            float p0 = -ms, p1 = -ms, y0, y1;
+                            ffma2(p0, p1, __uint_as_float(r[u][2 * c]), __uint_as_float(r[u][2 * c + 1]), k, k);
+                            p0 = kv_ex2(p0);
+                            p1 = kv_ex2(p1);
+                            fmul2(y0, y1, p0, p1, y, y);
+                            if (decltype(masked)::value) {
+                                const int t = key0 + 32 * j + 16 * u + 2 * c;
+                                if (t >= lim) p0 = y0 = 0.f;
+                                if (t + 1 >= lim) p1 = y1 = 0.f;
+                            }
+                            ffma2(add0, add1, p0, p1, 1.f, 1.f);
+                            kv_split(y0, y1, hi[c], lo[c]);
                         }
-                        ffma2(add0, add1, p0, p1, 1.f, 1.f);
-                        kv_split(y0, y1, hi[c], lo[c]);
+                        tmem_st8(ts + 32 * j + 16 * u, hi);
+                        tmem_st8(ts + 32 * j + 16 * u + 8, lo);
                     }
-                    tmem_st8(ts + 16 * j, hi);
-                    tmem_st8(ts + 16 * j + 8, lo);
+                    if (j & 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&bar_p[X][j >> 1]);
+                    }
                 }
+                tmem_ld_wait_dep(r[0]);
             };
             if (full) weigh(std::false_type{});
             else weigh(std::true_type{});
-            l = l * f + (add0 + add1);
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&bar_p[X]);
-            if (!mbar_wait(&bar_o_full[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
+            l += add0 + add1;
+        }
+        row_max[X][row] = m;  // (read by nobody but the sums' warps any more)
+        row_sum[X][row] = l;
+        if (row == 0) unit_exp[X] = E;
+        named_bar_sync(1, 384);
+    } else if (warp < 12) {
+        regs_inc<kRegsSum>();
+        const uint32_t to = tmem + lanes + kColO;
+        float o[D];
+        bool ok = true;
+#pragma unroll
+        for (int d = 0; d < D; d++) o[d] = 0.f;
+        for (int i = 0; i < n; i++) {
+            if (!mbar_wait(&bar_o_full[i & 1], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            {
-                uint32_t r[2][16];
-                tmem_ld16(to, r[0]);
+            const float g = row_gain[i & 3][row];
+            uint32_t r[2][16];
+            tmem_ld16(to, r[0]);
 #pragma unroll
-                for (int d = 0; d < D; d += 16) {
-                    tmem_ld_wait_dep(r[d / 16 & 1]);
-                    if (d + 16 < D) tmem_ld16(to + d + 16, r[(d / 16 + 1) & 1]);
+            for (int d = 0; d < D; d += 16) {
+                tmem_ld_wait_dep(r[d / 16 & 1]);
+                if (d + 16 < D) tmem_ld16(to + d + 16, r[(d / 16 + 1) & 1]);
 #pragma unroll
-                    for (int c = 0; c < 16; c++) o[d + c] = __fmaf_rn(o[d + c], g, __uint_as_float(r[d / 16 & 1][c]));
+                for (int c = 0; c < 16; c += 2) {
+                    float x = __uint_as_float(r[d / 16 & 1][c]), y = __uint_as_float(r[d / 16 & 1][c + 1]);
+                    ffma2(x, y, o[d + c], o[d + c + 1], g, g);
+                    o[d + c] = x;
+                    o[d + c + 1] = y;
                 }
             }
             tc_fence_before();
             mbar_arrive(&bar_o_empty);
         }
-        // the odd tiles' sums go through smem (free once every product is done) to the even tiles' threads
-        if (ok && n > 0) ok = mbar_wait(&bar_fin, 0, &abort_flag, status, kDevTimeoutTmemFull);
-        float* other = reinterpret_cast<float*>(smem) + row;  // [m, l, O[D]][128 rows]
-        const float back = kv_pow2(E - 15);
-        if (X == 1) {
-            other[0] = m;
-            other[kTileRows] = l;
-#pragma unroll
-            for (int d = 0; d < D; d++) other[(2 + d) * kTileRows] = o[d] * back;
-        }
-        named_bar_sync(1, 256);
-        if (X == 0 && ok && live) {
-            const float m1 = other[0], l1 = other[kTileRows], mn = fmaxf(m, m1), ms = mn == -INFINITY ? 0.f : mn;
-            const float f0 = kv_ex2(m - ms), f1 = kv_ex2(m1 - ms);
-            l = l * f0 + l1 * f1;
+        named_bar_sync(1, 384);
+        if (ok && live) {
+            const float m0 = row_max[0][row], m1 = row_max[1][row], mn = fmaxf(m0, m1), ms = mn == -INFINITY ? 0.f : mn;
+            const float l = row_sum[0][row] * kv_ex2(m0 - ms) + row_sum[1][row] * kv_ex2(m1 - ms);
             const bool none = mn == -INFINITY && l == 0.f;  // on the max too: a NaN sum stays NaN
             float* part = P.part + (((int64_t)split * P.tiles + gt) * a.c.H + h) * kTileRows * (D + 2);
             float* dst = a.out + out_row * a.ldo + (int64_t)head * D;
@@ -362,96 +387,108 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             } else if (P.lse) {
                 P.lse[out_row * a.heads + head] = none ? INFINITY : mn + log2f(l);
             }
-            const float c0 = f0 * back;
+            const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
 #pragma unroll
             for (int d = 0; d < D; d += 16) {
                 float x[16];
 #pragma unroll
-                for (int c = 0; c < 16; c++) x[c] = (o[d + c] * c0 + other[(2 + d + c) * kTileRows] * f1) * scale;
+                for (int c = 0; c < 16; c++) x[c] = o[d + c] * scale * back;
                 row_store(dst + d, x, vec);
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         regs_dec<kRegsConvert>();
-        const int cw = warp - 8, qn = lane / 4, qc = lane % 4;
-        uint4 kr[4 * J + (D % 64 ? 1 : 0)], vr[D / 16];
-        const uint32_t sb = smem_u32(smem);
-        // Blocks of key tile i: for K this warp's own; for V lanes of even and odd qn take the two blocks of the warp's
-        // half tile, so that eight lanes' 16-byte stores fall in different banks.  Past the cache's end: its last
-        // block (masked).
-        const int bv = cw / 2 * 2 + ((qn ^ cw) & 1);
-        auto record = [&](int i, int b) { return recs + (int64_t)min((t0 + i) * (kTileKeys / kKvBlock) + b, a.c.nb - 1) * REC + lane * 16; };
-        auto load_k = [&](int i) {
-            const uint8_t* r = record(i, cw);
-#pragma unroll
-            for (int u = 0; u < 4 * J + (D % 64 ? 1 : 0); u++) kr[u] = *reinterpret_cast<const uint4*>(r + u * 512);
+        const int cw = warp - 12, qn = lane / 4, qc = lane % 4;
+        // each warp copies one block of a key tile; past the cache's end: its last block (masked)
+        auto issue = [&](int i) {
+            if (lane == 0) {
+                mbar_expect_tx(&bar_raw[i & 1], REC);
+                bulk_load(smem + M::RAW + (i & 1) * M::RAW_TILE + cw * REC,
+                          recs + (int64_t)min((t0 + i) * (kTileKeys / kKvBlock) + cw, a.c.nb - 1) * REC, REC, &bar_raw[i & 1]);
+            }
         };
-        auto load_v = [&](int i) {
-            const uint8_t* r = record(i, bv) + 32 * D;
-#pragma unroll
-            for (int u = 0; u < D / 16; u++) vr[u] = *reinterpret_cast<const uint4*>(r + u * 512);
+        // K: the warp's own block.  V: lanes of even and odd qn take the two blocks of the warp's half tile, so that eight
+        // lanes' 16-byte stores fall in different banks.
+        const int bv = cw / 2 * 2 + ((qn ^ cw) & 1);
+        const uint32_t sb = smem_u32(smem);
+        auto ld128 = [](uint32_t at) {
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+            return v;
         };
         auto st128 = [](uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
         };
-        if (n > 0) {
-            load_k(0);
-            load_v(0);
-        }
-        for (int i = 0; i < n; i++) {
+        int issued = min(n, 2);
+        for (int i = 0; i < issued; i++) issue(i);
+        int i = 0;
+        for (; i < n; i++) {
             const int B = i & 1;
-            const uint32_t ph = ((i >> 1) - 1) & 1, kb = sb + B * M::K_TILE, vb = sb + M::V + B * M::V_TILE;
+            const uint32_t ph = ((i >> 1) - 1) & 1, raw = sb + M::RAW + B * M::RAW_TILE + lane * 16;
+            if (!mbar_wait(&bar_raw[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) break;
             if (i > 1 && !mbar_wait(&bar_k_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
+            {
+                const uint32_t rk = raw + cw * REC, t = 8 * (qn / 2) + qn % 2;  // token of its block: t + 2 nt
+                const uint32_t kb = sb + B * M::K_TILE + (32 * cw + t) * 128;
+#pragma unroll 2
+                for (uint32_t nt = 0; nt < 4; nt++) {
+                    const uint32_t x = (t + 2 * nt) & 7;
 #pragma unroll
-            for (int nt = 0; nt < 4; nt++) {
-                const int t = 32 * cw + 8 * (qn / 2) + 2 * nt + qn % 2;  // row of the key tile
-#pragma unroll
-                for (int j = 0; j < J; j++) {
-                    const uint4 w = kr[nt * J + j];
-                    const uint32_t at = kb + j * M::K_PANEL + t * 128;
-                    st128(at + (((2 * qc) ^ (t & 7)) << 4), kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
-                    st128(at + (((2 * qc + 1) ^ (t & 7)) << 4), kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
-                }
-                if (D % 64) {
-                    const uint4 w = kr[4 * J];
-                    const uint32_t x = nt == 0 ? w.x : nt == 1 ? w.y : nt == 2 ? w.z : w.w;
-                    const uint32_t at = kb + J * M::K_PANEL + t * 128 + (((qc / 2) ^ (t & 7)) << 4) + qc % 2 * 8;
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(kv_half2_lo(x)), "r"(kv_half2_hi(x)) : "memory");
+                    for (int j = 0; j < J; j++) {
+                        const uint4 w = ld128(rk + (nt * J + j) * 512);
+                        const uint32_t at = kb + j * M::K_PANEL + nt * 256;
+                        st128(at + ((2 * qc ^ x) << 4), kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
+                        st128(at + (((2 * qc + 1) ^ x) << 4), kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
+                    }
+                    if (D % 64) {
+                        uint32_t w;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(rk + 4 * J * 512 + nt * 4) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(kb + J * M::K_PANEL + nt * 256 + ((qc / 2 ^ x) << 4) + qc % 2 * 8),
+                                     "r"(kv_half2_lo(w)), "r"(kv_half2_hi(w))
+                                     : "memory");
+                    }
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&bar_k_full[B]);
-            if (i + 1 < n) load_k(i + 1);
             if (i > 1 && !mbar_wait(&bar_v_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
-#pragma unroll
-            for (int np = 0; np < D / 16; np++) {
-                const uint4 w = vr[np];
-#pragma unroll
-                for (int f = 0; f < 2; f++) {
-                    const int ch = 8 * (2 * np + f) + qn;
-                    const uint32_t x = f ? w.z : w.x, y = f ? w.w : w.y;
-                    st128(vb + cw / 2 * M::V_PANEL + ch * 128 + (((4 * (bv & 1) + qc) ^ qn) << 4), kv_half2_lo(x), kv_half2_hi(x),
-                          kv_half2_lo(y), kv_half2_hi(y));
+            {
+                const uint32_t rv = raw + bv * REC + 32 * D;
+                const uint32_t vb = sb + M::V + B * M::V_TILE + cw / 2 * M::V_PANEL + qn * 128 + (((4 * (bv & 1) + qc) ^ qn) << 4);
+#pragma unroll 2
+                for (uint32_t np = 0; np < D / 16; np++) {  // channels 16 np + qn, + 8
+                    const uint4 w = ld128(rv + np * 512);
+                    st128(vb + np * 2048, kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
+                    st128(vb + np * 2048 + 1024, kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&bar_v_full[B]);
-            if (i + 1 < n) load_v(i + 1);
+            named_bar_sync(2, 128);  // the tile's codes are read by all four warps
+            if (i + 2 < n) {
+                issue(i + 2);
+                issued = i + 3;
+            }
         }
+        // after a timeout: give the copies still in flight a last, bounded chance to land
+        for (; i < issued; i++)
+            for (int k = 0; k < 1000 && !mbar_try_wait(&bar_raw[i & 1], (i >> 1) & 1); k++) {}
     } else {
         regs_dec<kRegsMma>();
-        if (warp == 12 && lane == 0 && n > 0) {
-            const uint32_t sb = smem_u32(smem);
+        if (warp == 16 && lane == 0 && n > 0) {
+            const uint64_t dk = desc128(smem_u32(smem)), dv = desc128(smem_u32(smem + M::V));  // + byte offset / 16
             auto qk = [&](int i) {
                 const int B = i & 1;
                 if (!mbar_wait(&bar_k_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
                 tc_fence_after();
-#pragma unroll
-                for (int lo = 1; lo >= 0; lo--)
+#pragma unroll 1
+                for (int lo = 1; lo >= 0; lo--) {
+                    const uint64_t b = dk + B * (M::K_TILE / 16);
+                    const uint32_t q0 = tmem + kColQ + lo * (D / 2);
 #pragma unroll
                     for (int k = 0; k < D / 16; k++)
-                        mma_f16_ta(tmem + kColS + B * 128, tmem + kColQ + lo * (D / 2) + k * 8,
-                                   desc128(sb + B * M::K_TILE + k / 4 * M::K_PANEL + k % 4 * 32), IDESC_S, !lo || k);
+                        mma_f16_ta(tmem + kColS + B * 128, q0 + k * 8, b + (k / 4 * M::K_PANEL + k % 4 * 32) / 16, IDESC_S, !lo || k);
+                }
                 mma_commit(&bar_s[B]);
                 mma_commit(&bar_k_empty[B]);
                 return true;
@@ -460,20 +497,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 const int B = i & 1;
                 if (!mbar_wait(&bar_v_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
                 if (i > 0 && !mbar_wait(&bar_o_empty, (i - 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
-                if (!mbar_wait(&bar_p[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
-                tc_fence_after();
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    if (!mbar_wait(&bar_p[B][half], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
+                    tc_fence_after();
+                    const uint64_t b = dv + (B * M::V_TILE + half * M::V_PANEL) / 16;
+                    const uint32_t p0 = tmem + kColS + B * 128 + half * 64;
 #pragma unroll
-                for (int lo = 1; lo >= 0; lo--)
+                    for (int lo = 1; lo >= 0; lo--)
 #pragma unroll
-                    for (int k = 0; k < kTileKeys / 16; k++)
-                        mma_f16_ta(tmem + kColO, tmem + kColS + B * 128 + k * 16 + lo * 8,
-                                   desc128(sb + M::V + B * M::V_TILE + k / 4 * M::V_PANEL + k % 4 * 32), IDESC_O, !lo || k);
+                        for (int k = 0; k < kTileKeys / 32; k++)
+                            mma_f16_ta(tmem + kColO, p0 + k * 16 + lo * 8, b + k * 2, IDESC_O, half || !lo || k);
+                }
                 mma_commit(&bar_o_full[B]);
                 mma_commit(&bar_v_empty[B]);
                 return true;
             };
-            bool ok = qk(0) && (n < 2 || qk(1));
-            for (int i = 0; ok && i < n; i++) ok = pv(i) && (i + 2 >= n || qk(i + 2));
+            bool ok = qk(0);
+            for (int i = 1; ok && i <= n; i++) ok = (i == n || qk(i)) && pv(i - 1);
             // nothing of this CTA may still run when its TMEM is freed
             mma_commit(&bar_fin);
             for (int i = 0; i < 2000 && !mbar_try_wait(&bar_fin, 0); i++) {}
@@ -483,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 // Joins the key splits: one warp per pair of a (tile, head).
