@@ -157,7 +157,8 @@ __device__ __forceinline__ void kv_split(float a, float b, uint32_t& hi, uint32_
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = kv_pack(a - f.x, b - f.y);
+    ffma2(a, b, f.x, f.y, -1.f, -1.f);
+    lo = kv_pack(a, b);
 }
 
 // Tokens that row i of sequence q sees.

@@ -35,8 +35,8 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kTileRows = 128;   // pairs per CTA
 constexpr int kTileKeys = 128;
-// registers per thread by role: 128 x (2 x 104 + 168 + 80 + 24) = 640 x 96, what the launch has
-constexpr uint32_t kRegsSoftmax = 104, kRegsSum = 168, kRegsConvert = 80, kRegsMma = 24;
+// registers per thread by role: 128 x (2 x 104 + 168 + 48 + 56) = 640 x 96, what the launch has
+constexpr uint32_t kRegsSoftmax = 104, kRegsSum = 168, kRegsConvert = 48, kRegsMma = 56;
 
 template <int D>
 struct PromptSmem {
@@ -71,6 +71,13 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // 16 consecutive floats of a row
 __device__ __forceinline__ void row_load(const float* p, float (&x)[16], bool vec)
@@ -265,8 +272,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                         tmem_ld_wait_dep(r[u]);
                         tmem_ld16(ts + (32 * j + 16 * u + 16) % kTileKeys, r[u ^ 1]);
 #pragma unroll
-                        for (int c = 0; c < 16; c++)
-                            if (!decltype(masked)::value || key0 + 32 * j + 16 * u + c < lim) mx = fmaxf(mx, __uint_as_float(r[u][c]));
+                        for (int c = 0; c < 16; c += 2) {
+                            float x0 = __uint_as_float(r[u][c]), x1 = __uint_as_float(r[u][c + 1]);
+                            if (decltype(masked)::value) {
+                                const int t = key0 + 32 * j + 16 * u + c;
+                                if (t >= lim) x0 = -INFINITY;
+                                if (t + 1 >= lim) x1 = -INFINITY;
+                            }
+                            mx = max3(mx, x0, x1);
+                        }
                     }
                     const float k = coef * __shfl_sync(0xffffffffu, sc.x, j);
                     if (!decltype(masked)::value || mx != -INFINITY) mt = fmaxf(mt, mx * k);
