@@ -49,7 +49,7 @@ struct PromptSmem {
     static constexpr int RAW = V + 2 * V_TILE;
     static constexpr int BYTES = RAW + 2 * RAW_TILE + 1024;   // + alignment
 };
-// TMEM columns
+// TMEM columns; a CTA takes all 512, so they are addresses too
 constexpr uint32_t kColS = 0, kColO = 256, kColQ = 384;
 
 __device__ __forceinline__ uint64_t desc128(uint32_t saddr) { return smem_desc(saddr, 16, 1024, 2); }
@@ -192,7 +192,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    if (tmem_slot != 0 && tid == 0) {  // (the whole of TMEM begins at 0)
+        abort_flag = 1;
+        atomicCAS(a.status, 0u, (uint32_t)kDevBadTmem);
+    }
     const int X = warp / 4, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     int lim = 0, head = 0;
@@ -228,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 if (live) row_load(src + d, x, vec);
 #pragma unroll
                 for (int i = 0; i < 8; i++) kv_split(live ? x[2 * i] * up : 0.f, live ? x[2 * i + 1] * up : 0.f, hi[i], lo[i]);
-                tmem_st8(tmem + lanes + kColQ + d / 2, hi);
-                tmem_st8(tmem + lanes + kColQ + D / 2 + d / 2, lo);
+                tmem_st8(lanes + kColQ + d / 2, hi);
+                tmem_st8(lanes + kColQ + D / 2 + d / 2, lo);
             }
             tmem_st_wait();
         }
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
 
     if (warp < 8) {
         regs_inc<kRegsSoftmax>();
-        const uint32_t ts = tmem + lanes + kColS + X * 128;
+        const uint32_t ts = lanes + kColS + X * 128;
         float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
         int E = -100;                  // P_i holds p (dv / 2^(E - 15))
         // lane j < 4: the scales of key tile i's block j; blocks past the end hold anything
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         named_bar_sync(1, 384);
     } else if (warp < 12) {
         regs_inc<kRegsSum>();
-        const uint32_t to = tmem + lanes + kColO;
+        const uint32_t to = lanes + kColO;
         float o[D];
         bool ok = true;
 #pragma unroll
@@ -489,48 +492,60 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             for (int k = 0; k < 1000 && !mbar_try_wait(&bar_raw[i & 1], (i >> 1) & 1); k++) {}
     } else {
         regs_dec<kRegsMma>();
-        if (warp == 16 && lane == 0 && n > 0) {
+        if (warp == 16 && n > 0) {
+            // The warp stays together and one lane issues: operands are then known to be the same for all lanes and
+            // live in uniform registers.
+            const bool one = elect_one();
             const uint64_t dk = desc128(smem_u32(smem)), dv = desc128(smem_u32(smem + M::V));  // + byte offset / 16
-            auto qk = [&](int i) {
-                const int B = i & 1;
+            auto qk = [&](int i, auto parity) {
+                constexpr int B = decltype(parity)::value;
                 if (!mbar_wait(&bar_k_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
                 tc_fence_after();
-#pragma unroll 1
-                for (int lo = 1; lo >= 0; lo--) {
-                    const uint64_t b = dk + B * (M::K_TILE / 16);
-                    const uint32_t q0 = tmem + kColQ + lo * (D / 2);
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++)
-                        mma_f16_ta(tmem + kColS + B * 128, q0 + k * 8, b + (k / 4 * M::K_PANEL + k % 4 * 32) / 16, IDESC_S, !lo || k);
-                }
-                mma_commit(&bar_s[B]);
-                mma_commit(&bar_k_empty[B]);
-                return true;
-            };
-            auto pv = [&](int i) {
-                const int B = i & 1;
-                if (!mbar_wait(&bar_v_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
-                if (i > 0 && !mbar_wait(&bar_o_empty, (i - 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
-#pragma unroll 1
-                for (int half = 0; half < 2; half++) {
-                    if (!mbar_wait(&bar_p[B][half], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
-                    tc_fence_after();
-                    const uint64_t b = dv + (B * M::V_TILE + half * M::V_PANEL) / 16;
-                    const uint32_t p0 = tmem + kColS + B * 128 + half * 64;
+                if (one) {
 #pragma unroll
                     for (int lo = 1; lo >= 0; lo--)
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 32; k++)
-                            mma_f16_ta(tmem + kColO, p0 + k * 16 + lo * 8, b + k * 2, IDESC_O, half || !lo || k);
+                        for (int k = 0; k < D / 16; k++)
+                            mma_f16_ta(kColS + B * 128, kColQ + lo * (D / 2) + k * 8,
+                                       dk + (B * M::K_TILE + k / 4 * M::K_PANEL + k % 4 * 32) / 16, IDESC_S, !lo || k);
+                    mma_commit(&bar_s[B]);
+                    mma_commit(&bar_k_empty[B]);
                 }
-                mma_commit(&bar_o_full[B]);
-                mma_commit(&bar_v_empty[B]);
+                __syncwarp();
                 return true;
             };
-            bool ok = qk(0);
-            for (int i = 1; ok && i <= n; i++) ok = (i == n || qk(i)) && pv(i - 1);
+            auto pv = [&](int i, auto parity) {
+                constexpr int B = decltype(parity)::value;
+                if (!mbar_wait(&bar_v_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
+                if (i > 0 && !mbar_wait(&bar_o_empty, (i - 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    if (!mbar_wait(&bar_p[B][half], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
+                    tc_fence_after();
+                    if (one) {
+#pragma unroll
+                        for (int lo = 1; lo >= 0; lo--)
+#pragma unroll
+                            for (int k = 0; k < kTileKeys / 32; k++)
+                                mma_f16_ta(kColO, kColS + B * 128 + half * 64 + k * 16 + lo * 8,
+                                           dv + (B * M::V_TILE + half * M::V_PANEL) / 16 + k * 2, IDESC_O, half || !lo || k);
+                        if (half) {
+                            mma_commit(&bar_o_full[B]);
+                            mma_commit(&bar_v_empty[B]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                return true;
+            };
+            using Even = std::integral_constant<int, 0>;
+            using Odd = std::integral_constant<int, 1>;
+            bool ok = qk(0, Even{});
+#pragma unroll 1
+            for (int i = 0; ok && i < n; i += 2)
+                ok = (i + 1 >= n || qk(i + 1, Odd{})) && pv(i, Even{}) && (i + 2 >= n || qk(i + 2, Even{})) && (i + 1 >= n || pv(i + 1, Odd{}));
             // nothing of this CTA may still run when its TMEM is freed
-            mma_commit(&bar_fin);
+            if (one) mma_commit(&bar_fin);
             for (int i = 0; i < 2000 && !mbar_try_wait(&bar_fin, 0); i++) {}
         }
         __syncwarp();
@@ -538,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 16) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem_slot, 512);
 }
 
 // Joins the key splits: one warp per pair of a (tile, head).
