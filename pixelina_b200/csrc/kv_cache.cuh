@@ -72,11 +72,18 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& c, const int32_t* starts, 
 }
 
 // sum[s] = f(0) + .. + f(s - 1) for s <= S, computed by the whole CTA
-// (blockDim.x a multiple of 32, at most 1024); ends with a barrier.
+// (blockDim.x a multiple of 32, at most 1024); ends with a barrier.  f may be
+// evaluated by any number of threads.
 template <typename F>
 __device__ __forceinline__ void kv_prefix(int S, int* sum, int* warp_sums, F f)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    if (S == 1) {
+        const int x = f(0);
+        if (tid == 0) sum[0] = 0, sum[1] = x;
+        __syncthreads();
+        return;
+    }
     int carry = 0;
     for (int base = 0; base < S; base += blockDim.x) {
         const int s = base + tid;

@@ -79,31 +79,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
-// 16 consecutive floats of a row
-__device__ __forceinline__ void row_load(const float* p, float (&x)[16], bool vec)
-{
-#pragma unroll
-    for (int c = 0; c < 16; c += 4) {
-        if (vec) {
-            const float4 v = *reinterpret_cast<const float4*>(p + c);
-            x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
-        } else {
-            x[c] = p[c], x[c + 1] = p[c + 1], x[c + 2] = p[c + 2], x[c + 3] = p[c + 3];
-        }
-    }
-}
-__device__ __forceinline__ void row_store(float* p, const float (&x)[16], bool vec)
-{
-#pragma unroll
-    for (int c = 0; c < 16; c += 4) {
-        if (vec) {
-            *reinterpret_cast<float4*>(p + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
-        } else {
-            p[c] = x[c], p[c + 1] = x[c + 1], p[c + 2] = x[c + 2], p[c + 3] = x[c + 3];
-        }
-    }
-}
-
 struct PromptParams {
     KvAttnCall a;
     float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], O[128][D]
@@ -167,6 +142,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         mbar_init(&bar_fin, 1);
         fence_mbar_init();
     }
+    if (warp == 16) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
     griddep_wait();
     griddep_launch_dependents();
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
@@ -174,76 +154,88 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         if (blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
         return prompt_tiles(a, s);
     });
-    if (gt >= sum[a.c.S]) return;
-    const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-    const int pairs = q.n * G;
-    int t0, t1;
-    prompt_keys(a, q, tile, split, P.splits, t0, t1);
-    const int n = t1 - t0;
-    const int64_t sh = (int64_t)s * a.c.H + h;
-    const uint8_t* recs = a.c.codes + sh * a.c.nb * (int64_t)REC;
-    const float2* scales = a.c.scales + sh * a.c.nb;
-
-    if (warp == 16) {
-        tmem_alloc(&tmem_slot, 512);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
     tc_fence_after();
     if (tmem_slot != 0 && tid == 0) {  // (the whole of TMEM begins at 0)
         abort_flag = 1;
         atomicCAS(a.status, 0u, (uint32_t)kDevBadTmem);
     }
-    const int X = warp / 4, row = tid & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    int lim = 0, head = 0;
-    int64_t out_row = 0;
-    float coef = 0.f;
-    bool live = false;
-    if (warp < 12) {
-        const int p = tile * kTileRows + row;
-        live = p < pairs;
-        out_row = q.row0 + (live ? p / G : 0);
-        head = h * G + (live ? p % G : 0);
-        lim = live ? kv_limit(a, q, p / G) : 0;
+    uint32_t* status = a.status;
+    int n = 0, t0 = 0, tile = 0;
+    KvSeq q{};
+    int64_t sh = 0;
+    if (gt < sum[a.c.S]) {
+        const int s = kv_find(sum, a.c.S, gt);
+        tile = gt - sum[s];
+        q = kv_seq(a.c, a.starts, a.rows, s);
+        int t1;
+        prompt_keys(a, q, tile, split, P.splits, t0, t1);
+        n = t1 - t0;  // key tiles
+        sh = (int64_t)s * a.c.H + h;
     }
-    if (warp < 8) {  // the rows' queries: scaled to below 2^15, split, stored by the first four warps
-        const float* src = a.q + out_row * a.ldq + (int64_t)head * D;
+    const int pairs = q.n * G, tile0 = tile * kTileRows;
+    const uint8_t* recs = a.c.codes + sh * a.c.nb * (int64_t)REC;
+    const float2* scales = a.c.scales + sh * a.c.nb;
+    // codes of key tile i: converter warp cw copies one of its blocks; past the cache's end: its last block (masked)
+    auto copy_codes = [&](int i, int cw) {
+        mbar_expect_tx(&bar_raw[i & 1], REC);
+        bulk_load(smem + M::RAW + (i & 1) * M::RAW_TILE + cw * REC,
+                  recs + (int64_t)min((t0 + i) * (kTileKeys / kKvBlock) + cw, a.c.nb - 1) * REC, REC, &bar_raw[i & 1]);
+    };
+    if (warp >= 12 && warp < 16 && lane == 0)
+        for (int i = 0; i < min(n, 2); i++) copy_codes(i, warp - 12);
+    // the rows' queries, through smem where K and V will be: whole rows in, a row per thread out
+    constexpr int QP = D + 4;
+    static_assert(kTileRows * QP * 4 <= M::RAW, "rows fit where K and V will be");
+    float* rows = reinterpret_cast<float*>(smem);
+    {
         const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
+        for (int r = warp; r < kTileRows && lane < D / 4; r += kThreads / 32) {
+            const int p = tile0 + r;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p < pairs) {
+                const float* src = a.q + (int64_t)(q.row0 + p / G) * a.ldq + (int64_t)(h * G + p % G) * D + 4 * lane;
+                if (vec) x = *reinterpret_cast<const float4*>(src);
+                else x = make_float4(src[0], src[1], src[2], src[3]);
+            }
+            *reinterpret_cast<float4*>(rows + r * QP + 4 * lane) = x;
+        }
+    }
+    __syncthreads();
+    const int X = warp / 4, row = tid & 127, p = tile0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float coef = 0.f;
+    if (warp < 8) {  // scaled to below 2^15, split, stored: the two warpgroups take turns
+        const float* src = rows + row * QP;
         float m = 0.f;
-#pragma unroll 2
-        for (int d = 0; d < D; d += 16) {
-            float x[16];
-            if (live) row_load(src + d, x, vec);
-#pragma unroll
-            for (int i = 0; i < 16; i++) m = live ? fmaxf(m, fabsf(x[i])) : 0.f;
+#pragma unroll 4
+        for (int d = 0; d < D; d += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src + d);
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
         }
         const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(m))) : 0;
         const float up = kv_pow2(e);
         coef = kv_log2_inv_sqrt(D) * kv_pow2(-e);
-        if (X == 0) {
-#pragma unroll 2
-            for (int d = 0; d < D; d += 16) {
-                float x[16];
-                uint32_t hi[8], lo[8];
-                if (live) row_load(src + d, x, vec);
+#pragma unroll 1
+        for (int d = 16 * X; d < D; d += 32) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) kv_split(live ? x[2 * i] * up : 0.f, live ? x[2 * i + 1] * up : 0.f, hi[i], lo[i]);
-                tmem_st8(lanes + kColQ + d / 2, hi);
-                tmem_st8(lanes + kColQ + D / 2 + d / 2, lo);
+            for (int i = 0; i < 4; i++) {
+                const float4 x = *reinterpret_cast<const float4*>(src + d + 4 * i);
+                kv_split(x.x * up, x.y * up, hi[2 * i], lo[2 * i]);
+                kv_split(x.z * up, x.w * up, hi[2 * i + 1], lo[2 * i + 1]);
             }
-            tmem_st_wait();
+            tmem_st8(lanes + kColQ + d / 2, hi);
+            tmem_st8(lanes + kColQ + D / 2 + d / 2, lo);
         }
+        tmem_st_wait();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    uint32_t* status = a.status;
 
     if (warp < 8) {
         regs_inc<kRegsSoftmax>();
+        const int lim = p < pairs ? kv_limit(a, q, p / G) : 0;
         const uint32_t ts = lanes + kColS + X * 128;
         float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
         int E = -100;                  // P_i holds p (dv / 2^(E - 15))
@@ -387,43 +379,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_arrive(&bar_o_empty);
         }
         named_bar_sync(1, 384);
-        if (ok && live) {
+        if (ok && gt < sum[a.c.S]) {
             const float m0 = row_max[0][row], m1 = row_max[1][row], mn = fmaxf(m0, m1), ms = mn == -INFINITY ? 0.f : mn;
             const float l = row_sum[0][row] * kv_ex2(m0 - ms) + row_sum[1][row] * kv_ex2(m1 - ms);
             const bool none = mn == -INFINITY && l == 0.f;  // on the max too: a NaN sum stays NaN
+            const bool whole = P.splits == 1;
             float* part = P.part + (((int64_t)split * P.tiles + gt) * a.c.H + h) * kTileRows * (D + 2);
-            float* dst = a.out + out_row * a.ldo + (int64_t)head * D;
-            bool vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0;
-            float scale = none ? 0.f : __fdiv_rn(1.f, l);
-            if (P.splits > 1) {
+            if (!whole) {
                 part[row] = mn;
                 part[kTileRows + row] = l;
-                dst = part + 2 * kTileRows + (int64_t)row * D;
-                vec = true;
-                scale = 1.f;
-            } else if (P.lse) {
-                P.lse[out_row * a.heads + head] = none ? INFINITY : mn + log2f(l);
+            } else if (P.lse && p < pairs) {
+                P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] = none ? INFINITY : mn + log2f(l);
             }
-            const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
+            const float scale = (none ? 0.f : whole ? __fdiv_rn(1.f, l) : 1.f), back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
+            // through smem again (every product is done): a row per thread in, whole rows out
+            float* src = rows + row * QP;
 #pragma unroll
-            for (int d = 0; d < D; d += 16) {
-                float x[16];
-#pragma unroll
-                for (int c = 0; c < 16; c++) x[c] = o[d + c] * scale * back;
-                row_store(dst + d, x, vec);
+            for (int d = 0; d < D; d += 4)
+                *reinterpret_cast<float4*>(src + d) = make_float4(o[d] * scale * back, o[d + 1] * scale * back, o[d + 2] * scale * back,
+                                                                  o[d + 3] * scale * back);
+            __syncwarp();
+            const bool vec = !whole || ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0);
+            if (lane < D / 4) {
+                const int r0 = (warp & 3) * 32;
+                int t = (tile0 + r0) / G, g = (tile0 + r0) % G;
+#pragma unroll 4
+                for (int r = r0; r < min(r0 + 32, pairs - tile0); r++) {
+                    float* dst = whole ? a.out + (int64_t)(q.row0 + t) * a.ldo + (int64_t)(h * G + g) * D
+                                       : part + 2 * kTileRows + (int64_t)r * D;
+                    if (++g == G) g = 0, t++;
+                    const float4 x = *reinterpret_cast<const float4*>(rows + r * QP + 4 * lane);
+                    dst += 4 * lane;
+                    if (vec) *reinterpret_cast<float4*>(dst) = x;
+                    else dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
+                }
             }
         }
     } else if (warp < 16) {
         regs_dec<kRegsConvert>();
         const int cw = warp - 12, qn = lane / 4, qc = lane % 4;
-        // each warp copies one block of a key tile; past the cache's end: its last block (masked)
-        auto issue = [&](int i) {
-            if (lane == 0) {
-                mbar_expect_tx(&bar_raw[i & 1], REC);
-                bulk_load(smem + M::RAW + (i & 1) * M::RAW_TILE + cw * REC,
-                          recs + (int64_t)min((t0 + i) * (kTileKeys / kKvBlock) + cw, a.c.nb - 1) * REC, REC, &bar_raw[i & 1]);
-            }
-        };
         // K: the warp's own block.  V: lanes of even and odd qn take the two blocks of the warp's half tile, so that eight
         // lanes' 16-byte stores fall in different banks.
         const int bv = cw / 2 * 2 + ((qn ^ cw) & 1);
@@ -436,9 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         auto st128 = [](uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
         };
-        int issued = min(n, 2);
-        for (int i = 0; i < issued; i++) issue(i);
-        int i = 0;
+        int issued = min(n, 2), i = 0;
         for (; i < n; i++) {
             const int B = i & 1;
             const uint32_t ph = ((i >> 1) - 1) & 1, raw = sb + M::RAW + B * M::RAW_TILE + lane * 16;
@@ -483,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_arrive(&bar_v_full[B]);
             named_bar_sync(2, 128);  // the tile's codes are read by all four warps
             if (i + 2 < n) {
-                issue(i + 2);
+                if (lane == 0) copy_codes(i + 2, cw);
                 issued = i + 3;
             }
         }
