@@ -1463,6 +1463,7 @@ int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t r
     a.starts = starts;
     a.max_rows = (int64_t)max_rows;
     a.heads = (int)heads;
+    a.G = (int)heads / c->v.H;
     a.causal = causal ? 1 : 0;
     a.weights = weights;
     a.weights_out = weights_out;

@@ -64,7 +64,7 @@ struct QFrag {
 
     __device__ __forceinline__ void load(const KvAttnCall& a, const KvSeq& q, int h, int tile)
     {
-        const int lane = lane_id(), r = lane / 4, c = lane % 4, G = a.heads / a.c.H, pairs = q.n * G;
+        const int lane = lane_id(), r = lane / 4, c = lane % 4, G = a.G, pairs = q.n * G;
 #pragma unroll
         for (int u = 0; u < PT / 8; u++) {
             const int p = tile * PT + r + 8 * u;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ 
     __shared__ uint32_t abort_flag;
     const KvAttnCall& a = P.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane / 4, c = lane % 4;
-    const int tile = blockIdx.y, G = a.heads / a.c.H;
+    const int tile = blockIdx.y, G = a.G;
     uint8_t* ring = dyn + warp * NST * REC;
     float* comb = reinterpret_cast<float*>(dyn);  // at a segment's end, in each warp's ring: m[PT], l[PT], O[PT][D]
     if (tid == 0) abort_flag = 0;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ Attn
     griddep_wait();
     griddep_launch_dependents();
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * a.c.H; });
-    const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.heads / a.c.H;
+    const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.G;
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
     const int nb = (sum[s + 1] - sum[s]) / a.c.H;
     if (nb == 0 || gp >= q.n * G) return;
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
 {
     const KvAttnCall& a = P.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
-    const int s = blockIdx.z, h = blockIdx.y, b = blockIdx.x * AW + warp, G = a.heads / a.c.H;
+    const int s = blockIdx.z, h = blockIdx.y, b = blockIdx.x * AW + warp, G = a.G;
     griddep_wait();
     griddep_launch_dependents();
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
@@ -482,7 +482,7 @@ struct AttnPlan {
 AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
 {
     AttnPlan p{};
-    const int64_t pairs = a.max_rows * (a.heads / a.c.H);
+    const int64_t pairs = a.max_rows * a.G;
     p.pt = pairs <= 8 ? 8 : 16;
     p.tiles = (int)((pairs + p.pt - 1) / p.pt);
     p.runs = num_sms;
@@ -501,7 +501,7 @@ cudaError_t launch_split(const AttnParams& P, const AttnPlan& p, cudaStream_t s)
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_attn<D, PT>, dim3((unsigned)p.runs, (unsigned)p.tiles), dim3(AW * 32), smem, s, P);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_kv_combine<D, PT>, dim3((unsigned)(P.a.max_rows * (P.a.heads / P.a.c.H)), (unsigned)P.a.c.H, (unsigned)P.a.c.S),
+    return launch_pdl(k_kv_combine<D, PT>, dim3((unsigned)(P.a.max_rows * P.a.G), (unsigned)P.a.c.H, (unsigned)P.a.c.S),
                       dim3(128), 0, s, P);
 }
 

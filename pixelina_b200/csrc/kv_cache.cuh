@@ -64,7 +64,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& c, const int32_t* starts, 
         q.row0 = a;
         q.n = (a < 0 || b < a || b > rows) ? -1 : b - a;
     } else {
-        const int n = (int)(rows / c.S);
+        const int n = (int)rows / c.S;
         q.row0 = s * n;
         q.n = n;
     }

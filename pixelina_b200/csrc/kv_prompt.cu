@@ -64,6 +64,11 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uin
         ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -90,17 +95,17 @@ __device__ __forceinline__ int prompt_tiles(const KvAttnCall& a, int s)
 {
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
     if (q.n <= 0 || q.n > a.max_rows) return 0;
-    return (int)(((int64_t)q.n * (a.heads / a.c.H) + kTileRows - 1) / kTileRows);
+    return (q.n * a.G + kTileRows - 1) / kTileRows;  // (the host checks that rows x G fits)
 }
 
 // The part of a (sequence, head)'s keys that a split of one CTA takes:
 // key tiles [t0, t1) of those that the tile's last row sees.
 __device__ __forceinline__ void prompt_keys(const KvAttnCall& a, const KvSeq& q, int tile, int split, int splits, int& t0, int& t1)
 {
-    const int G = a.heads / a.c.H, pairs = q.n * G;
+    const int G = a.G, pairs = q.n * G;
     const int last = min(pairs, (tile + 1) * kTileRows) - 1;
     const int lim = kv_limit(a, q, last / G);
-    const int n = (lim + kTileKeys - 1) / kTileKeys, per = (n + splits - 1) / splits;
+    const int n = (lim + kTileKeys - 1) / kTileKeys, per = splits == 1 ? n : (n + splits - 1) / splits;
     t0 = min(n, split * per);
     t1 = min(n, t0 + per);
 }
@@ -115,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
     __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_s[2], bar_m[2], bar_p[2][2], bar_o_full[2],
-        bar_o_empty, bar_fin;
+        bar_o_empty, bar_rows, bar_q, bar_fin;
     __shared__ float row_max[2][kTileRows], row_sum[2][kTileRows], row_gain[4][kTileRows];  // by tile's parity; gain by tile % 4
     __shared__ int unit_exp[2];
     __shared__ uint32_t tmem_slot, abort_flag;
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
 
     const KvAttnCall& a = P.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int h = blockIdx.x % a.c.H, gt = P.tiles - 1 - blockIdx.x / a.c.H, split = blockIdx.y, G = a.heads / a.c.H;
+    const int h = blockIdx.x % a.c.H, gt = P.tiles - 1 - blockIdx.x / a.c.H, split = blockIdx.y, G = a.G;
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < 2; i++) {
@@ -139,6 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_init(&bar_o_full[i], 1);
         }
         mbar_init(&bar_o_empty, 128);
+        mbar_init(&bar_rows, 128);
+        mbar_init(&bar_q, 256);
         mbar_init(&bar_fin, 1);
         fence_mbar_init();
     }
@@ -173,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         sh = (int64_t)s * a.c.H + h;
     }
     const int pairs = q.n * G, tile0 = tile * kTileRows;
+    float* part = P.part + (((int64_t)split * P.tiles + gt) * a.c.H + h) * kTileRows * (D + 2);  // (splits > 1)
     const uint8_t* recs = a.c.codes + sh * a.c.nb * (int64_t)REC;
     const float2* scales = a.c.scales + sh * a.c.nb;
     // codes of key tile i: converter warp cw copies one of its blocks; past the cache's end: its last block (masked)
@@ -183,58 +191,64 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     };
     if (warp >= 12 && warp < 16 && lane == 0)
         for (int i = 0; i < min(n, 2); i++) copy_codes(i, warp - 12);
-    // the rows' queries, through smem where K and V will be: whole rows in, a row per thread out
-    constexpr int QP = D + 4;
-    static_assert(kTileRows * QP * 4 <= M::RAW, "rows fit where K and V will be");
-    float* rows = reinterpret_cast<float*>(smem);
-    {
-        const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
-        for (int r = warp; r < kTileRows && lane < D / 4; r += kThreads / 32) {
-            const int p = tile0 + r;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p < pairs) {
-                const float* src = a.q + (int64_t)(q.row0 + p / G) * a.ldq + (int64_t)(h * G + p % G) * D + 4 * lane;
-                if (vec) x = *reinterpret_cast<const float4*>(src);
-                else x = make_float4(src[0], src[1], src[2], src[3]);
-            }
-            *reinterpret_cast<float4*>(rows + r * QP + 4 * lane) = x;
-        }
-    }
-    __syncthreads();
     const int X = warp / 4, row = tid & 127, p = tile0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    float coef = 0.f;
-    if (warp < 8) {  // scaled to below 2^15, split, stored: the two warpgroups take turns
-        const float* src = rows + row * QP;
-        float m = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(src + d);
-            m = fmaxf(fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-        }
-        const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(m))) : 0;
-        const float up = kv_pow2(e);
-        coef = kv_log2_inv_sqrt(D) * kv_pow2(-e);
-#pragma unroll 1
-        for (int d = 16 * X; d < D; d += 32) {
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 x = *reinterpret_cast<const float4*>(src + d + 4 * i);
-                kv_split(x.x * up, x.y * up, hi[2 * i], lo[2 * i]);
-                kv_split(x.z * up, x.w * up, hi[2 * i + 1], lo[2 * i + 1]);
-            }
-            tmem_st8(lanes + kColQ + d / 2, hi);
-            tmem_st8(lanes + kColQ + D / 2 + d / 2, lo);
-        }
-        tmem_st_wait();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    // rows of q at first, and of the result at last, stand where the second K tile and V are in between
+    float* const mine = reinterpret_cast<float*>(smem + M::K_TILE) + row * (D + 4);
+    static_assert(kTileRows * (D + 4) * 4 <= M::RAW - M::K_TILE, "rows fit");
 
     if (warp < 8) {
         regs_inc<kRegsSoftmax>();
+        // the row's query: one bulk copy (or, unaligned, plain loads), then scaled to below 2^15, split, stored in TMEM;
+        // the two warpgroups take half of the channels each
+        const bool bulk = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
+        float4 x[D / 8];
+        {
+            const float* src = a.q + (int64_t)(q.row0 + p / G) * a.ldq + (int64_t)(h * G + p % G) * D;
+            if (bulk) {
+                if (X == 0) {
+                    if (p < pairs) {
+                        mbar_expect_tx(&bar_rows, D * 4);
+                        bulk_load(mine, src, D * 4, &bar_rows);
+                    } else {
+                        mbar_arrive(&bar_rows);
+                    }
+                }
+                mbar_wait(&bar_rows, 0, &abort_flag, status, kDevTimeoutFull);
+            }
+            src += X * (D / 2);
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) {
+                if (p >= pairs) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                else if (bulk) x[i] = *reinterpret_cast<const float4*>(mine + X * (D / 2) + 4 * i);
+                else x[i] = make_float4(src[4 * i], src[4 * i + 1], src[4 * i + 2], src[4 * i + 3]);
+            }
+        }
+        float coef;
+        {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) top = max3(max3(top, fabsf(x[i].x), fabsf(x[i].y)), fabsf(x[i].z), fabsf(x[i].w));
+            row_sum[X][row] = top;
+            named_bar_sync(3, 256);
+            top = fmaxf(top, row_sum[X ^ 1][row]);
+            const int e = top > 0.f && top <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(top))) : 0;
+            const float up = kv_pow2(e);
+            coef = kv_log2_inv_sqrt(D) * kv_pow2(-e);
+#pragma unroll
+            for (int i = 0; i < D / 8; i += 2) {
+                uint32_t hi[4], lo[4];
+                kv_split(x[i].x * up, x[i].y * up, hi[0], lo[0]);
+                kv_split(x[i].z * up, x[i].w * up, hi[1], lo[1]);
+                kv_split(x[i + 1].x * up, x[i + 1].y * up, hi[2], lo[2]);
+                kv_split(x[i + 1].z * up, x[i + 1].w * up, hi[3], lo[3]);
+                tmem_st4(lanes + kColQ + X * (D / 4) + 2 * i, hi);
+                tmem_st4(lanes + kColQ + D / 2 + X * (D / 4) + 2 * i, lo);
+            }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bar_q);
         const int lim = p < pairs ? kv_limit(a, q, p / G) : 0;
         const uint32_t ts = lanes + kColS + X * 128;
         float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
@@ -379,40 +393,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_arrive(&bar_o_empty);
         }
         named_bar_sync(1, 384);
-        if (ok && gt < sum[a.c.S]) {
+        if (ok) {
             const float m0 = row_max[0][row], m1 = row_max[1][row], mn = fmaxf(m0, m1), ms = mn == -INFINITY ? 0.f : mn;
             const float l = row_sum[0][row] * kv_ex2(m0 - ms) + row_sum[1][row] * kv_ex2(m1 - ms);
             const bool none = mn == -INFINITY && l == 0.f;  // on the max too: a NaN sum stays NaN
-            const bool whole = P.splits == 1;
-            float* part = P.part + (((int64_t)split * P.tiles + gt) * a.c.H + h) * kTileRows * (D + 2);
-            if (!whole) {
+            if (P.splits > 1 && p < pairs) {
                 part[row] = mn;
                 part[kTileRows + row] = l;
             } else if (P.lse && p < pairs) {
                 P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] = none ? INFINITY : mn + log2f(l);
             }
-            const float scale = (none ? 0.f : whole ? __fdiv_rn(1.f, l) : 1.f), back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
-            // through smem again (every product is done): a row per thread in, whole rows out
-            float* src = rows + row * QP;
+            const float scale = none ? 0.f : P.splits > 1 ? 1.f : __fdiv_rn(1.f, l);
+            const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
+            // every product is done: the row goes through smem, out by one bulk copy (or, unaligned, plain stores)
+            float* dst = P.splits > 1 ? part + 2 * kTileRows + (int64_t)row * D : a.out + (int64_t)(q.row0 + p / G) * a.ldo + (int64_t)(h * G + p % G) * D;
+            if (P.splits > 1 || ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0)) {
 #pragma unroll
-            for (int d = 0; d < D; d += 4)
-                *reinterpret_cast<float4*>(src + d) = make_float4(o[d] * scale * back, o[d + 1] * scale * back, o[d + 2] * scale * back,
-                                                                  o[d + 3] * scale * back);
-            __syncwarp();
-            const bool vec = !whole || ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0);
-            if (lane < D / 4) {
-                const int r0 = (warp & 3) * 32;
-                int t = (tile0 + r0) / G, g = (tile0 + r0) % G;
-#pragma unroll 4
-                for (int r = r0; r < min(r0 + 32, pairs - tile0); r++) {
-                    float* dst = whole ? a.out + (int64_t)(q.row0 + t) * a.ldo + (int64_t)(h * G + g) * D
-                                       : part + 2 * kTileRows + (int64_t)r * D;
-                    if (++g == G) g = 0, t++;
-                    const float4 x = *reinterpret_cast<const float4*>(rows + r * QP + 4 * lane);
-                    dst += 4 * lane;
-                    if (vec) *reinterpret_cast<float4*>(dst) = x;
-                    else dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
-                }
+                for (int d = 0; d < D; d += 4)
+                    *reinterpret_cast<float4*>(mine + d) = make_float4(o[d] * scale * back, o[d + 1] * scale * back, o[d + 2] * scale * back,
+                                                                       o[d + 3] * scale * back);
+                fence_proxy_async_smem();
+                if (p < pairs) bulk_store(dst, mine, D * 4);
+                bulk_commit();
+                bulk_wait_read_all();
+            } else if (p < pairs) {
+#pragma unroll
+                for (int d = 0; d < D; d++) dst[d] = o[d] * scale * back;
             }
         }
     } else if (warp < 16) {
@@ -460,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             }
             fence_proxy_async_smem();
             mbar_arrive(&bar_k_full[B]);
+            if (i == 0 && !mbar_wait(&bar_q, 0, &abort_flag, status, kDevTimeoutEmpty)) break;  // the queries have left V's place and K's second
             if (i > 1 && !mbar_wait(&bar_v_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
             {
                 const uint32_t rv = raw + bv * REC + 32 * D;
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             };
             using Even = std::integral_constant<int, 0>;
             using Odd = std::integral_constant<int, 1>;
-            bool ok = qk(0, Even{});
+            bool ok = mbar_wait(&bar_q, 0, &abort_flag, status, kDevTimeoutFull) && qk(0, Even{});
 #pragma unroll 1
             for (int i = 0; ok && i < n; i += 2)
                 ok = (i + 1 >= n || qk(i + 1, Odd{})) && pv(i, Even{}) && (i + 2 >= n || qk(i + 2, Even{})) && (i + 1 >= n || pv(i + 1, Odd{}));
@@ -558,7 +565,7 @@ __global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptP
     griddep_wait();
     griddep_launch_dependents();
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles(a, s); });
-    const int gt = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, G = a.heads / a.c.H;
+    const int gt = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, G = a.G;
     if (gt >= sum[a.c.S]) return;
     const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
@@ -603,7 +610,7 @@ struct PromptPlan {
 PromptPlan plan_prompt(const KvAttnCall& a, int num_sms)
 {
     PromptPlan p{};
-    const int64_t G = a.heads / a.c.H;
+    const int64_t G = a.G;
     // a sequence's n rows make at most n G / 128 + 1 tiles
     const int64_t most = std::min<int64_t>(a.c.S * ((a.max_rows * G + kTileRows - 1) / kTileRows), a.rows * G / kTileRows + a.c.S);
     p.tiles = (int)most;
@@ -621,7 +628,7 @@ cudaError_t launch_d(const PromptParams& P, cudaStream_t s)
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_prompt<D>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
     if (e != cudaSuccess || P.splits == 1) return e;
-    const int64_t pairs = std::min<int64_t>(kTileRows, P.a.max_rows * (P.a.heads / P.a.c.H));
+    const int64_t pairs = std::min<int64_t>(kTileRows, P.a.max_rows * P.a.G);
     return launch_pdl(k_kv_join<D>, dim3((unsigned)P.tiles, (unsigned)P.a.c.H, (unsigned)((pairs + 7) / 8)), dim3(256), 0, s, P);
 }
 

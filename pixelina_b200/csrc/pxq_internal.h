@@ -211,6 +211,7 @@ struct KvAttnCall {
     const int32_t* starts;   // device [S + 1], or null: rows / S rows each
     int64_t max_rows;        // most rows of one sequence
     int heads;
+    int G;                   // heads / kv heads
     int causal;
     const float* weights;    // [S][H][cap] running totals, may be null (zero)
     float* weights_out;      // null: no weights wanted
