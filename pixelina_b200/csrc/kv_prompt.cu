@@ -35,8 +35,8 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kTileRows = 128;   // pairs per CTA
 constexpr int kTileKeys = 128;
-// registers per thread by role: 128 x (2 x 104 + 168 + 48 + 56) = 640 x 96, what the launch has
-constexpr uint32_t kRegsSoftmax = 104, kRegsSum = 168, kRegsConvert = 48, kRegsMma = 56;
+// registers per thread by role: 128 x (2 x 104 + 168 + 72 + 32) = 640 x 96, what the launch has
+constexpr uint32_t kRegsSoftmax = 104, kRegsSum = 168, kRegsConvert = 72, kRegsMma = 32;
 
 template <int D>
 struct PromptSmem {
@@ -445,21 +445,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             {
                 const uint32_t rk = raw + cw * REC, t = 8 * (qn / 2) + qn % 2;  // token of its block: t + 2 nt
                 const uint32_t kb = sb + B * M::K_TILE + (32 * cw + t) * 128;
-#pragma unroll 2
-                for (uint32_t nt = 0; nt < 4; nt++) {
-                    const uint32_t x = (t + 2 * nt) & 7;
+                // four loads at a time: one load's latency covers 80 instructions
 #pragma unroll
-                    for (int j = 0; j < J; j++) {
-                        const uint4 w = ld128(rk + (nt * J + j) * 512);
-                        const uint32_t at = kb + j * M::K_PANEL + nt * 256;
-                        st128(at + ((2 * qc ^ x) << 4), kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
-                        st128(at + (((2 * qc + 1) ^ x) << 4), kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
+                for (uint32_t n0 = 0; n0 < 4; n0 += 4 / J) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) w[u] = ld128(rk + (n0 * J + u) * 512);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const uint32_t nt = n0 + u / J, x = (t + 2 * nt) & 7, at = kb + u % J * M::K_PANEL + nt * 256;
+                        st128(at + ((2 * qc ^ x) << 4), kv_half2_lo(w[u].x), kv_half2_hi(w[u].x), kv_half2_lo(w[u].y), kv_half2_hi(w[u].y));
+                        st128(at + (((2 * qc + 1) ^ x) << 4), kv_half2_lo(w[u].z), kv_half2_hi(w[u].z), kv_half2_lo(w[u].w), kv_half2_hi(w[u].w));
                     }
-                    if (D % 64) {
-                        uint32_t w;
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(rk + 4 * J * 512 + nt * 4) : "memory");
+                }
+                if (D % 64) {
+                    const uint4 r = ld128(rk + 4 * J * 512);
+                    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                    for (uint32_t nt = 0; nt < 4; nt++) {
+                        const uint32_t x = (t + 2 * nt) & 7;
                         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(kb + J * M::K_PANEL + nt * 256 + ((qc / 2 ^ x) << 4) + qc % 2 * 8),
-                                     "r"(kv_half2_lo(w)), "r"(kv_half2_hi(w))
+                                     "r"(kv_half2_lo(w[nt])), "r"(kv_half2_hi(w[nt]))
                                      : "memory");
                     }
                 }
@@ -471,11 +477,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             {
                 const uint32_t rv = raw + bv * REC + 32 * D;
                 const uint32_t vb = sb + M::V + B * M::V_TILE + cw / 2 * M::V_PANEL + qn * 128 + (((4 * (bv & 1) + qc) ^ qn) << 4);
-#pragma unroll 2
-                for (uint32_t np = 0; np < D / 16; np++) {  // channels 16 np + qn, + 8
-                    const uint4 w = ld128(rv + np * 512);
-                    st128(vb + np * 2048, kv_half2_lo(w.x), kv_half2_hi(w.x), kv_half2_lo(w.y), kv_half2_hi(w.y));
-                    st128(vb + np * 2048 + 1024, kv_half2_lo(w.z), kv_half2_hi(w.z), kv_half2_lo(w.w), kv_half2_hi(w.w));
+                constexpr int VG = D / 16 % 4 == 0 ? 4 : 5;
+                static_assert(D / 16 % VG == 0, "whole groups");
+#pragma unroll
+                for (uint32_t n0 = 0; n0 < D / 16; n0 += VG) {  // channels 16 np + qn, + 8
+                    uint4 w[VG];
+#pragma unroll
+                    for (int u = 0; u < VG; u++) w[u] = ld128(rv + (n0 + u) * 512);
+#pragma unroll
+                    for (int u = 0; u < VG; u++) {
+                        st128(vb + (n0 + u) * 2048, kv_half2_lo(w[u].x), kv_half2_hi(w[u].x), kv_half2_lo(w[u].y), kv_half2_hi(w[u].y));
+                        st128(vb + (n0 + u) * 2048 + 1024, kv_half2_lo(w[u].z), kv_half2_hi(w[u].z), kv_half2_lo(w[u].w), kv_half2_hi(w[u].w));
+                    }
                 }
             }
             fence_proxy_async_smem();
