@@ -13,7 +13,7 @@
 // leaves 2^-22 of the value; products and sums are fp32.  So the result is
 // that of an fp32 computation at two half-precision products per element.
 //
-//   k_kv_attn     split keys: one CTA per SM takes an equal run of the
+//   k_kv_attn     split keys: every CTA takes an equal run of the
 //                 flattened (sequence, head, block) list; warps take a run's
 //                 blocks in turn, each with its own running max and sum
 //   k_kv_combine  joins the parts of a (sequence, head) that spans CTAs
@@ -25,8 +25,9 @@
 namespace pxq {
 namespace {
 
-constexpr int AW = 8;                    // warps per CTA
-constexpr int kMinRun = 8;               // fewest blocks worth a CTA: one per warp
+constexpr int AW = 4;                    // warps per CTA
+constexpr int kCtasPerSm = 2;            // one joins its warps or waits for queries while the other streams
+constexpr int kMinRun = 4;               // fewest blocks worth a CTA: one per warp
 
 // D += A (16 x 16, row) * B (16 x 8, column), fp16 in, fp32 out
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -157,7 +158,7 @@ template <int D>
 constexpr size_t attn_smem_bytes() { return (size_t)AW * kAttnStages * kv_record_bytes(D); }
 
 template <int D, int PT>
-__global__ void __launch_bounds__(AW * 32, 1) k_kv_attn(const __grid_constant__ AttnParams P)
+__global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_constant__ AttnParams P)
 {
     constexpr int NST = kAttnStages, REC = kv_record_bytes(D), U = PT / 8, NT = D / 8;
     constexpr int CW = NST * REC / 4;  // floats between two warps' rings
@@ -485,7 +486,7 @@ AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
     const int64_t pairs = a.max_rows * a.G;
     p.pt = pairs <= 8 ? 8 : 16;
     p.tiles = (int)((pairs + p.pt - 1) / p.pt);
-    p.runs = num_sms;
+    p.runs = kCtasPerSm * num_sms;
     p.prompt = pairs > 16;
     if (p.prompt) p.part_bytes = (kv_prompt_part_bytes(a, num_sms) + 255) / 256 * 256;
     else p.part_bytes = ((size_t)p.tiles * p.runs * 2 * p.pt * (a.c.D + 2) * sizeof(float) + 255) / 256 * 256;

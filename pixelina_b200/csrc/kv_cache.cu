@@ -173,7 +173,6 @@ __global__ void __launch_bounds__(2 * D)
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
     __shared__ float2 red[2 * D / 32];
-    __shared__ uint32_t flag;
     const int tid = threadIdx.x, h = blockIdx.y;
     griddep_wait();
     griddep_launch_dependents();
@@ -181,17 +180,21 @@ __global__ void __launch_bounds__(2 * D)
     kv_prefix(c.S, sum, warp_sums, [&](int s) {
         const KvSeq q = kv_seq(c, starts, rows, s);
         bad |= q.n < 0;
+        kv_prefetch(c.slot + s);
         return kv_touched(c, q.len, q.n);
     });
+    const bool work = (int)blockIdx.x < sum[c.S];
+    const int s = work ? kv_find(sum, c.S, (int)blockIdx.x) : 0;
+    const KvSeq q = kv_seq(c, starts, rows, s);
+    const int slot = c.slot[s];
     bad = __syncthreads_or(bad);  // bounds outside the arrays: nothing is appended
-    if (!bad && (int)blockIdx.x < sum[c.S]) {
-        const int s = kv_find(sum, c.S, (int)blockIdx.x);
-        const KvSeq q = kv_seq(c, starts, rows, s);
+    bool last_reader = false;     // (used at the end: the atomic's latency passes meanwhile)
+    if (tid == 0) last_reader = kv_last_reader(c.ticket, gridDim.x * gridDim.y);
+    if (!bad && work) {
         const int b0 = q.len / kKvBlock, b = b0 + (int)blockIdx.x - sum[s], last = b0 + sum[s + 1] - sum[s] - 1;
         const int have = b == b0 ? q.len % kKvBlock : 0;                  // rows of the block already there
         const int64_t first = (int64_t)b * kKvBlock - q.len;              // new row index of the block's token 0
         const int end = (int)min((int64_t)kKvBlock, q.n - first);         // present rows
-        const int slot = c.slot[s];
         const int to = (q.len % kKvBlock != 0 && last != b0) ? slot ^ 1 : slot;
         const float* tk = kv_tail(c, s, slot, h, 0);
         const float* tv = kv_tail(c, s, slot, h, 1);
@@ -218,8 +221,8 @@ __global__ void __launch_bounds__(2 * D)
         }
         kv_store_block<D>(c, (int64_t)s * c.H + h, b, xk, xv, red);
     }
-    // every CTA has read the lengths: the last one advances them
-    if (!kv_last_cta(c.ticket, gridDim.x * gridDim.y, &flag)) return;
+    // every CTA has read the lengths: the last one to do so advances them
+    if (!__syncthreads_or(last_reader)) return;
     for (int s = tid; s < c.S; s += blockDim.x) {
         const KvSeq q = kv_seq(c, starts, rows, s);
         if (bad || q.n < 0) {
@@ -242,19 +245,21 @@ template <int D>
 __global__ void __launch_bounds__(2 * D) k_kv_truncate(const __grid_constant__ KvView c, const int32_t* lengths)
 {
     __shared__ float2 red[2 * D / 32];
-    __shared__ uint32_t flag;
     const int tid = threadIdx.x, h = blockIdx.x, s = blockIdx.y;
     griddep_wait();
     griddep_launch_dependents();
-    const int len = c.lens[s], to = lengths ? lengths[s] : 0;
+    const int len = c.lens[s], to = lengths ? lengths[s] : 0, slot = c.slot[s], holds = c.held[s];
+    __syncthreads();
+    bool last_reader = false;
+    if (tid == 0) last_reader = kv_last_reader(c.ticket, gridDim.x * gridDim.y);
     if (to >= 0 && to < len && to % kKvBlock != 0) {
         const int b = to / kKvBlock, end = to % kKvBlock;
         const int kt = tid / (D / 16), kc = tid % (D / 16), vd = tid % D, vt = tid / D;
-        float* tk = kv_tail(c, s, c.slot[s], h, 0);
-        float* tv = kv_tail(c, s, c.slot[s], h, 1);
+        float* tk = kv_tail(c, s, slot, h, 0);
+        float* tv = kv_tail(c, s, slot, h, 1);
         const int64_t sh = (int64_t)s * c.H + h;
         float xk[16], xv[16];
-        const bool held = c.held[s] == b;
+        const bool held = holds == b;
         if (held) {
             ld16(tk + kt * D + 16 * kc, xk, true);
 #pragma unroll
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(2 * D) k_kv_truncate(const __grid_constant__ K
         __syncthreads();  // every code of the block is read
         kv_store_block<D>(c, sh, b, xk, xv, red);
     }
-    if (!kv_last_cta(c.ticket, gridDim.x * gridDim.y, &flag)) return;
+    if (!__syncthreads_or(last_reader)) return;
     for (int i = tid; i < c.S; i += blockDim.x) {
         const int n = c.lens[i], t = lengths ? lengths[i] : 0;
         if (t < 0 || t >= n) continue;

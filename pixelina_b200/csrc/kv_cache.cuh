@@ -122,23 +122,17 @@ __device__ __forceinline__ int kv_find(const int* sum, int S, int u)
     return lo;
 }
 
-// Whether this CTA is the last of the grid to get here (all its earlier
-// writes are visible to that one); leaves the ticket at zero.
-__device__ __forceinline__ bool kv_last_cta(uint32_t* ticket, uint32_t ctas, uint32_t* flag)
+// Count this CTA as one that has read the lengths (called by one thread after
+// a barrier behind those reads).  Returns whether it is the last of the grid:
+// the one that may write them, as soon as it likes.  Leaves the ticket at zero.
+__device__ __forceinline__ bool kv_last_reader(uint32_t* ticket, uint32_t ctas)
 {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        const uint32_t t = atomicAdd(ticket, 1u);
-        *flag = t == ctas - 1;
-        if (t == ctas - 1) {
-            __threadfence();
-            *ticket = 0;
-        }
-    }
-    __syncthreads();
-    return *flag != 0;
+    const uint32_t t = atomicAdd(ticket, 1u);
+    if (t != ctas - 1) return false;
+    *ticket = 0;
+    return true;
 }
+__device__ __forceinline__ void kv_prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 
 __device__ __forceinline__ float kv_log2_inv_sqrt(int D) { return 1.4426950408889634f / sqrtf((float)D); }
 

@@ -175,9 +175,13 @@ def _torch():
 
 
 def _stream_ptr(stream=None):
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
     torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the current stream without a Stream object around it
+    if raw is not None:
+        return C.c_void_p(raw(torch.cuda.current_device()))
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
 def _ptr(t) -> C.c_void_p:
@@ -310,9 +314,12 @@ def attention(q, k, v, heads: int, kv_heads: int, ranges=None, query_offset: int
     return out
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(stream):
     """Tensors made within belong to the stream that the call runs on."""
-    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+    return _HERE if stream is None else _torch().cuda.stream(stream)
 
 
 def _rows(x, width: int, what: str, device):
