@@ -1341,6 +1341,39 @@ int check_kv(const pxq_kv_cache* c)
     return PXQ_OK;
 }
 
+// One call's scratch: small needs from the stream's buffer (work on one stream
+// is ordered), large ones and those of a captured call stream-ordered -- a
+// graph then has memory of its own, whatever else was captured on the stream.
+struct KvScratch {
+    void* ptr = nullptr;
+    cudaStream_t s = nullptr;
+    bool own = false;
+    int get(size_t need, cudaStream_t stream)
+    {
+        s = stream;
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        PXQ_CUDA(cudaStreamIsCapturing(stream, &st));
+        if (st == cudaStreamCaptureStatusNone && need <= ((size_t)8 << 20)) {
+            // past the matvec's counter region, which every call must leave zero
+            uint8_t* base = static_cast<uint8_t*>(stream_scratch(t_device, stream, kMvCounterRegion + need));
+            if (base) ptr = base + kMvCounterRegion;
+        }
+        if (!ptr) {
+            own = true;
+            if (cudaMallocAsync(&ptr, need, stream) != cudaSuccess) {
+                cudaGetLastError();
+                return fail(PXQ_ERR_NO_MEMORY, "scratch of %zu bytes", need);
+            }
+        }
+        return PXQ_OK;
+    }
+    void put()
+    {
+        if (own) cudaFreeAsync(ptr, s);
+        own = false;
+    }
+};
+
 // The packed rows of a batch: with no starts, every sequence has the same number.
 int check_kv_rows(const pxq_kv_cache* c, size_t rows, const int32_t* starts)
 {
@@ -1465,19 +1498,16 @@ int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t r
     a.heads = (int)heads;
     a.G = (int)heads / c->v.H;
     a.causal = causal ? 1 : 0;
+    a.qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 4 == 0;
+    a.ovec = reinterpret_cast<uintptr_t>(output) % 16 == 0 && ldo % 4 == 0;
     a.weights = weights;
     a.weights_out = weights_out;
     a.status = d->status;
-    // stream-ordered scratch: a captured call gets memory of its own graph
-    void* scratch = nullptr;
-    const size_t need = kv_attention_scratch_bytes(a, d->sms);
-    if (cudaMallocAsync(&scratch, need, s) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(PXQ_ERR_NO_MEMORY, "attention scratch of %zu bytes", need);
-    }
+    KvScratch scratch;
+    if (int rc = scratch.get(kv_attention_scratch_bytes(a, d->sms), s)) return rc;
     int launches = 0;
-    const cudaError_t e = launch_kv_attention(a, scratch, d->sms, s, &launches);
-    cudaFreeAsync(scratch, s);
+    const cudaError_t e = launch_kv_attention(a, scratch.ptr, d->sms, s, &launches);
+    scratch.put();
     if (counted(e, (uint64_t)launches) != cudaSuccess) return fail(PXQ_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
     return PXQ_OK;
 }
@@ -1497,17 +1527,13 @@ int pxq_kv_evict(const pxq_kv_cache* src, pxq_kv_cache* dst, const float* weight
     if (int rc = check_kv(src)) return rc;
     if (int rc = check_kv(dst)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    void* own = nullptr;
+    KvScratch scratch;
     if (!kept) {
-        const size_t need = (size_t)src->v.S * src->v.H * keep * sizeof(int32_t);
-        if (cudaMallocAsync(&own, need, s) != cudaSuccess) {
-            cudaGetLastError();
-            return fail(PXQ_ERR_NO_MEMORY, "eviction scratch of %zu bytes", need);
-        }
+        if (int rc = scratch.get((size_t)src->v.S * src->v.H * keep * sizeof(int32_t), s)) return rc;
+        kept = static_cast<int32_t*>(scratch.ptr);
     }
-    const cudaError_t e = launch_kv_evict(src->v, dst->v, weights, (int64_t)keep, (int64_t)recent, weights_out,
-                                          own ? static_cast<int32_t*>(own) : kept, s);
-    if (own) cudaFreeAsync(own, s);
+    const cudaError_t e = launch_kv_evict(src->v, dst->v, weights, (int64_t)keep, (int64_t)recent, weights_out, kept, s);
+    scratch.put();
     if (counted(e, 2) != cudaSuccess) return fail(PXQ_ERR_CUDA, "eviction launch failed: %s", cudaGetErrorString(e));
     return PXQ_OK;
 }

@@ -73,15 +73,27 @@ struct QFrag {
             const float* src = a.q + (int64_t)(q.row0 + (live ? p / G : 0)) * a.ldq + (int64_t)(h * G + (live ? p % G : 0)) * D;
             float m = 0.f;
             float x[D / 16][4];
+            auto fetch = [&](auto vec) {
 #pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                const int d = k < D / 64 * 4 ? 64 * (k / 4) + 16 * c + 4 * (k % 4) : D / 64 * 64 + 4 * c;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[k][i] = live ? src[d + i] : 0.f;
-                    m = fmaxf(m, fabsf(x[k][i]));
+                for (int k = 0; k < D / 16; k++) {
+                    const int d = k < D / 64 * 4 ? 64 * (k / 4) + 16 * c + 4 * (k % 4) : D / 64 * 64 + 4 * c;
+                    float4 v;
+                    if (decltype(vec)::value) v = *reinterpret_cast<const float4*>(src + d);
+                    else v = make_float4(src[d], src[d + 1], src[d + 2], src[d + 3]);
+                    x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
                 }
+            };
+            if (!live) {
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
+            } else if (a.qvec) {
+                fetch(std::true_type{});
+            } else {
+                fetch(std::false_type{});
             }
+#pragma unroll
+            for (int k = 0; k < D / 16; k++)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(x[k][0]), fabsf(x[k][1])), fmaxf(fabsf(x[k][2]), fabsf(x[k][3]))));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // |x| 2^e < 2^15; a row of zeros, or one that is not finite, stays as it is
@@ -192,7 +204,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
     for (int w = w0; w < w1;) {
         const int s = kv_find(sum, a.c.S, w);
         const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-        const int nb = kv_attn_blocks(a, s);
+        const int nb = max(1, (q.len + kKvBlock - 1) / kKvBlock);
         const int h = (w - sum[s]) / nb, seg = sum[s] + h * nb;  // this (sequence, head)'s blocks: [seg, seg + nb)
         const int b0 = w - seg, b1 = min(seg + nb, w1) - seg;
         const bool first = b0 > 0, whole = b0 == 0 && b1 == nb;
@@ -346,34 +358,39 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             }
         }
         __syncthreads();
+        // every thread the same: each warp's weight for each of its pairs, then four channels at a time
         float* part = P.part + (((int64_t)tile * P.runs + blockIdx.x) * 2 + (first ? 0 : 1)) * PT * (D + 2);
-        for (int x = tid; x < PT * D; x += AW * 32) {
-            const int p = x / D, d = x % D, gp = tile * PT + p;
-            float M = -INFINITY;
+        constexpr int TPP = AW * 32 / PT;  // threads per pair
+        const int pr = tid / TPP, gp = tile * PT + pr;
+        float f[AW], M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int i = 0; i < AW; i++) M = fmaxf(M, comb[i * CW + p]);
-            const float Ms = M == -INFINITY ? 0.f : M;
-            float L = 0.f, O = 0.f;
+        for (int i = 0; i < AW; i++) M = fmaxf(M, f[i] = comb[i * CW + pr]);
+        const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
-            for (int i = 0; i < AW; i++) {
-                const float* src = comb + i * CW;
-                const float f = kv_ex2(src[p] - Ms);
-                L += src[PT + p] * f;
-                O += src[2 * PT + p * D + d] * f;
+        for (int i = 0; i < AW; i++) {
+            f[i] = kv_ex2(f[i] - Ms);
+            L += comb[i * CW + PT + pr] * f[i];
+        }
+        if (gp < pairs) {
+            const bool none = M == -INFINITY && L == 0.f;  // no token seen; the max is asked too, so that a NaN sum stays NaN
+            const int64_t row = q.row0 + gp / G;
+            const int head = h * G + gp % G;
+            float* dst = whole ? a.out + row * a.ldo + (int64_t)head * D : part + 2 * PT + pr * D;
+            const float scale = none ? 0.f : whole ? __fdiv_rn(1.f, L) : 1.f;
+            if (tid % TPP == 0) {
+                if (!whole) part[pr] = M, part[PT + pr] = L;
+                else if (P.lse) P.lse[row * a.heads + head] = none ? INFINITY : M + log2f(L);
             }
-            if (gp >= pairs) continue;
-            if (whole) {
-                const int64_t row = q.row0 + gp / G;
-                const int head = h * G + gp % G;
-                // no token seen: zeros.  The test is on the max, so that a NaN sum stays NaN.
-                a.out[row * a.ldo + (int64_t)head * D + d] = M == -INFINITY && L == 0.f ? 0.f : O / L;
-                if (P.lse && d == 0) P.lse[row * a.heads + head] = M == -INFINITY && L == 0.f ? INFINITY : M + log2f(L);
-            } else {
-                part[2 * PT + x] = O;
-                if (d == 0) {
-                    part[p] = M;
-                    part[PT + p] = L;
+            for (int d = 4 * (tid % TPP); d < D; d += 4 * TPP) {
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < AW; i++) {
+                    const float4 v = *reinterpret_cast<const float4*>(comb + i * CW + 2 * PT + pr * D + d);
+                    y.x += v.x * f[i], y.y += v.y * f[i], y.z += v.z * f[i], y.w += v.w * f[i];
                 }
+                y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
+                if (!whole || a.ovec) *reinterpret_cast<float4*>(dst + d) = y;
+                else dst[d] = y.x, dst[d + 1] = y.y, dst[d + 2] = y.z, dst[d + 3] = y.w;
             }
         }
         fence_proxy_async_smem();  // the next segment's copies follow these writes
@@ -390,9 +407,11 @@ __global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ Attn
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
     const KvAttnCall& a = P.a;
+    // The kernel before lets this one start once its own wait for its predecessors is over, so what those wrote (the
+    // lengths, the starts) may be read already; its own results may not.
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * a.c.H; });
     griddep_wait();
     griddep_launch_dependents();
-    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * a.c.H; });
     const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.G;
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
     const int nb = (sum[s + 1] - sum[s]) / a.c.H;
@@ -405,9 +424,11 @@ __global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ Attn
         return P.part + (((int64_t)tile * P.runs + cta) * 2 + (cta == c0 && seg >= cta * run ? 1 : 0)) * PT * (D + 2);
     };
     float M = -INFINITY;
+#pragma unroll 8
     for (int i = c0; i <= c1; i++) M = fmaxf(M, part(i)[p]);
     const float Ms = M == -INFINITY ? 0.f : M;
     float L = 0.f, O = 0.f;
+#pragma unroll 8
     for (int i = c0; i <= c1; i++) {
         const float* src = part(i);
         const float f = kv_ex2(src[p] - Ms);
@@ -498,7 +519,8 @@ template <int D, int PT>
 cudaError_t launch_split(const AttnParams& P, const AttnPlan& p, cudaStream_t s)
 {
     constexpr size_t smem = attn_smem_bytes<D>();
-    cudaError_t e = cudaFuncSetAttribute(k_kv_attn<D, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint32_t> done{0};
+    cudaError_t e = allow_smem(k_kv_attn<D, PT>, (int)smem, done);
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_attn<D, PT>, dim3((unsigned)p.runs, (unsigned)p.tiles), dim3(AW * 32), smem, s, P);
     if (e != cudaSuccess) return e;

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         regs_inc<kRegsSoftmax>();
         // the row's query: one bulk copy (or, unaligned, plain loads), then scaled to below 2^15, split, stored in TMEM;
         // the two warpgroups take half of the channels each
-        const bool bulk = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 4 == 0;
+        const bool bulk = a.qvec != 0;
         float4 x[D / 8];
         {
             const float* src = a.q + (int64_t)(q.row0 + p / G) * a.ldq + (int64_t)(h * G + p % G) * D;
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
             // every product is done: the row goes through smem, out by one bulk copy (or, unaligned, plain stores)
             float* dst = P.splits > 1 ? part + 2 * kTileRows + (int64_t)row * D : a.out + (int64_t)(q.row0 + p / G) * a.ldo + (int64_t)(h * G + p % G) * D;
-            if (P.splits > 1 || ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0)) {
+            if (P.splits > 1 || a.ovec) {
 #pragma unroll
                 for (int d = 0; d < D; d += 4)
                     *reinterpret_cast<float4*>(mine + d) = make_float4(o[d] * scale * back, o[d + 1] * scale * back, o[d + 2] * scale * back,
@@ -637,7 +637,8 @@ template <int D>
 cudaError_t launch_d(const PromptParams& P, cudaStream_t s)
 {
     constexpr int smem = PromptSmem<D>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(k_kv_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint32_t> done{0};
+    cudaError_t e = allow_smem(k_kv_prompt<D>, smem, done);
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_prompt<D>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
     if (e != cudaSuccess || P.splits == 1) return e;

@@ -1,5 +1,6 @@
 // pxq_internal.h -- declarations shared by the pxq translation units.
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda.h>
@@ -160,6 +161,18 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// cudaFuncAttributeMaxDynamicSharedMemorySize of `kernel`, set once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint32_t>& done)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 32 && (done.load(std::memory_order_acquire) >> dev & 1u))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 32) done.fetch_or(1u << dev, std::memory_order_release);
+    return e;
+}
+
 // ---- attention.cu ----------------------------------------------------------
 // fp32 multi-head attention with the semantics of tensor_attention
 // (src/tensor.cpp:347-427): q/out [q_rows][heads*head_dim], k/v
@@ -213,6 +226,7 @@ struct KvAttnCall {
     int heads;
     int G;                   // heads / kv heads
     int causal;
+    int qvec, ovec;          // q, out: every row starts on 16 bytes
     const float* weights;    // [S][H][cap] running totals, may be null (zero)
     float* weights_out;      // null: no weights wanted
     uint32_t* status;

@@ -323,23 +323,26 @@ def _on(stream):
 
 
 def _rows(x, width: int, what: str, device):
-    """An fp32 matrix of `width` columns on `device` whose rows may be strided."""
+    """An fp32 matrix of `width` columns on `device` whose rows may be strided,
+    and its row stride (of one row: its width, whatever torch says)."""
     torch = _torch()
-    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != width or x.device != device:
+    if x.dtype is not torch.float32 or x.dim() != 2 or x.shape[1] != width or x.device != device:
         raise ValueError(f"{what} must be fp32 [rows, {width}] on {device}")
-    return x if x.stride(1) == 1 and x.stride(0) >= width else x.contiguous()
+    if x.is_contiguous():
+        return x, width
+    ld, step = x.stride()
+    if step != 1 or ld < width:
+        return x.contiguous(), width
+    return x, ld if x.shape[0] > 1 else width
 
 
 def _whole(x, shape, dtype, what: str, device):
-    """A contiguous tensor of this shape and type on `device`, or None."""
-    if x is not None and (tuple(x.shape) != tuple(shape) or x.dtype != dtype or not x.is_contiguous() or x.device != device):
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
-    return x
-
-
-def _ld(x) -> int:
-    """Row stride of a matrix (one row: its width, whatever torch says)."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    """Address of a contiguous tensor of this shape and type on `device`; None for None."""
+    if x is None:
+        return None
+    if x.shape != shape or x.dtype is not dtype or not x.is_contiguous() or x.device != device:
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {shape} on {device}")
+    return x.data_ptr()
 
 
 class KVCache:
@@ -357,7 +360,7 @@ class KVCache:
             self.memory = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
         self.device = self.memory.device
         h = C.c_void_p()
-        _check(lib.pxq_kv_cache_create(_ptr(self.memory), sequences, capacity, kv_heads, head_dim, C.byref(h), _stream_ptr(stream)))
+        _check(lib.pxq_kv_cache_create(self.memory.data_ptr(), sequences, capacity, kv_heads, head_dim, C.byref(h), _stream_ptr(stream)))
         self.handle = h
 
     def release(self) -> None:
@@ -377,14 +380,14 @@ class KVCache:
         return self.handle
 
     def _per_sequence(self, x, what: str, more: int = 0):
-        return _whole(x, (self.sequences + more,), _torch().int32, what, self.device)
+        return None if x is None else _whole(x, (self.sequences + more,), _torch().int32, what, self.device)
 
     def lengths(self, stream=None):
         """The sequences' lengths: int32 cuda tensor."""
         h = self._live()
         with _on(stream):
             out = _torch().empty(self.sequences, dtype=_torch().int32, device=self.device)
-        _check(load().pxq_kv_cache_lengths(h, _ptr(out), _stream_ptr(stream)))
+        _check(load().pxq_kv_cache_lengths(h, out.data_ptr(), _stream_ptr(stream)))
         return out
 
     def append(self, k, v, starts=None, stream=None) -> None:
@@ -392,15 +395,16 @@ class KVCache:
         h = self._live()
         width = self.kv_heads * self.head_dim
         with _on(stream):
-            k, v = _rows(k, width, "k", self.device), _rows(v, width, "v", self.device)
+            k, ldk = _rows(k, width, "k", self.device)
+            v, ldv = _rows(v, width, "v", self.device)
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-        _check(load().pxq_kv_append(h, _ptr(k), _ld(k), _ptr(v), _ld(v), k.shape[0], _ptr(self._per_sequence(starts, "starts", 1)),
+        _check(load().pxq_kv_append(h, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0], self._per_sequence(starts, "starts", 1),
                                     _stream_ptr(stream)))
 
     def truncate(self, lengths=None, stream=None) -> None:
         """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them)."""
-        _check(load().pxq_kv_truncate(self._live(), _ptr(self._per_sequence(lengths, "lengths")), _stream_ptr(stream)))
+        _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), _stream_ptr(stream)))
 
     def read(self, first=None, count: Optional[int] = None, k=None, v=None, stream=None):
         """The values of tokens [first[s], first[s] + count) of every sequence:
@@ -410,10 +414,12 @@ class KVCache:
         h = self._live()
         count = self.capacity if count is None else count
         shape = (self.sequences, count, self.kv_heads * self.head_dim)
-        with _on(stream):
-            k, v = (torch.zeros(shape, device=self.device) if x is None else _whole(x, shape, torch.float32, what, self.device)
-                    for x, what in ((k, "k"), (v, "v")))
-        _check(load().pxq_kv_read(h, _ptr(self._per_sequence(first, "first")), count, _ptr(k), _ptr(v), _stream_ptr(stream)))
+        if k is None or v is None:
+            with _on(stream):
+                k = torch.zeros(shape, device=self.device) if k is None else k
+                v = torch.zeros(shape, device=self.device) if v is None else v
+        _check(load().pxq_kv_read(h, self._per_sequence(first, "first"), count, _whole(k, shape, torch.float32, "k", self.device),
+                                  _whole(v, shape, torch.float32, "v", self.device), _stream_ptr(stream)))
         return k, v
 
 
@@ -424,20 +430,25 @@ def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[
     (None: no bound but rows).  weights_out = weights + what each cached token
     received, [sequences, kv_heads, capacity]."""
     torch = _torch()
-    h = cache._live()
+    h, device = cache._live(), cache.device
     width = heads * cache.head_dim
     with _on(stream):
-        q = _rows(q, width, "q", cache.device)
-        rows = q.shape[0]
+        q, ldq = _rows(q, width, "q", device)
+        rows, ldo = q.shape[0], width
         if out is None:
-            out = torch.empty((rows, width), dtype=torch.float32, device=cache.device)
-    if tuple(out.shape) != (rows, width) or out.dtype != torch.float32 or out.device != cache.device or out.stride(1) != 1 or _ld(out) < width:
-        raise ValueError(f"out must be fp32 [{rows}, {width}] on {cache.device}, its rows contiguous")
-    shape = (cache.sequences, cache.kv_heads, cache.capacity)
-    _whole(weights, shape, torch.float32, "weights", cache.device)
-    _whole(weights_out, shape, torch.float32, "weights_out", cache.device)
-    _check(load().pxq_kv_attention(h, _ptr(q), _ld(q), rows, _ptr(cache._per_sequence(starts, "starts", 1)), max_rows or rows, heads,
-                                   1 if causal else 0, _ptr(out), _ld(out), _ptr(weights), _ptr(weights_out), _stream_ptr(stream)))
+            out = torch.empty((rows, width), dtype=torch.float32, device=device)
+        elif out.shape != (rows, width) or out.dtype is not torch.float32 or out.device != device or out.stride(1) != 1 or \
+                (rows > 1 and out.stride(0) < width):
+            raise ValueError(f"out must be fp32 [{rows}, {width}] on {device}, its rows contiguous")
+        elif rows > 1:
+            ldo = out.stride(0)
+    wi = wo = None
+    if weights is not None or weights_out is not None:
+        shape = (cache.sequences, cache.kv_heads, cache.capacity)
+        wi = _whole(weights, shape, torch.float32, "weights", device)
+        wo = _whole(weights_out, shape, torch.float32, "weights_out", device)
+    _check(load().pxq_kv_attention(h, q.data_ptr(), ldq, rows, cache._per_sequence(starts, "starts", 1), max_rows or rows, heads,
+                                   1 if causal else 0, out.data_ptr(), ldo, wi, wo, _stream_ptr(stream)))
     return out
 
 
@@ -450,10 +461,10 @@ def kv_evict(src: KVCache, dst: KVCache, weights, keep: Optional[int] = None, re
     keep = dst.capacity if keep is None else keep
     if weights is None:
         raise ValueError("weights are needed")
-    _whole(weights, (src.sequences, src.kv_heads, src.capacity), torch.float32, "weights", src.device)
-    _whole(weights_out, (dst.sequences, dst.kv_heads, dst.capacity), torch.float32, "weights_out", src.device)
-    _whole(kept, (src.sequences, src.kv_heads, keep), torch.int32, "kept", src.device)
-    _check(load().pxq_kv_evict(a, b, _ptr(weights), keep, recent, _ptr(weights_out), _ptr(kept), _stream_ptr(stream)))
+    heads = (src.sequences, src.kv_heads)
+    _check(load().pxq_kv_evict(a, b, _whole(weights, heads + (src.capacity,), torch.float32, "weights", src.device), keep, recent,
+                               _whole(weights_out, (dst.sequences, dst.kv_heads, dst.capacity), torch.float32, "weights_out", src.device),
+                               _whole(kept, heads + (keep,), torch.int32, "kept", src.device), _stream_ptr(stream)))
 
 
 class _Uploaded:
