@@ -545,16 +545,12 @@ cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms,
     P.lse = p.lse_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + p.part_bytes) : nullptr;
     P.runs = p.runs;
     if (p.prompt) {
-        const cudaError_t e = launch_kv_prompt(a, P.part, P.lse, num_sms, s, launches);
-        if (e != cudaSuccess || !a.weights_out) return e;
-        ++*launches;
-    } else {
-        *launches = a.weights_out ? 3 : 2;
+        return launch_kv_prompt(a, P.part, P.lse, num_sms, s, launches);
     }
+    *launches = a.weights_out ? 3 : 2;
     return by_dim(a.c.D, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        cudaError_t e = cudaSuccess;
-        if (!p.prompt) e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
+        cudaError_t e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
         if (e != cudaSuccess || !a.weights_out) return e;
         return launch_pdl(k_kv_weights<D>, dim3((unsigned)((a.c.nb + AW - 1) / AW), (unsigned)a.c.H, (unsigned)a.c.S), dim3(AW * 32), 0,
                           s, P);

@@ -19,6 +19,13 @@
 // S_{i+2} may overwrite P_i because the products of one thread are executed
 // in the order in which it issues them.
 //
+// With W the kernel finds the weight that each token received instead: the
+// rows' maxima and sums being known (lse), p = exp2(S coef dk - lse) is summed
+// over the tile's 128 pairs, first over a warp's rows (lane j ends up with
+// column j), then over the four warps; k_kv_weight_sum adds the tiles up in
+// their order.  No atomics: the result does not depend on the order of
+// execution.
+//
 // The tensor core cuts the accumulator's last bits at every K = 16 step, always
 // towards zero, and over a long sum that adds up: with one accumulator for a
 // whole prompt of 4096 tokens (256 steps on average) the output was off by
@@ -89,6 +96,10 @@ struct PromptParams {
     float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], O[128][D]
     float* lse;
     int tiles, splits;
+    // weights (W): pair tiles [tile0, tile0 + tiles) of the batch; sums over a tile's pairs go to wpart [tile][head][wkeys]
+    int tile0;
+    float* wpart;
+    int64_t wkeys;
 };
 
 __device__ __forceinline__ int prompt_tiles(const KvAttnCall& a, int s)
@@ -110,7 +121,7 @@ __device__ __forceinline__ void prompt_keys(const KvAttnCall& a, const KvSeq& q,
     t1 = min(n, t0 + per);
 }
 
-template <int D>
+template <int D, bool W>
 __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant__ PromptParams P)
 {
     using M = PromptSmem<D>;
@@ -119,16 +130,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     extern __shared__ uint8_t dyn[];
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
-    __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_s[2], bar_m[2], bar_p[2][2], bar_o_full[2],
+    __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_raw_empty[2], bar_s[2], bar_m[2], bar_w[2], bar_p[2][2], bar_o_full[2],
         bar_o_empty, bar_rows, bar_q, bar_fin;
     __shared__ float row_max[2][kTileRows], row_sum[2][kTileRows], row_gain[4][kTileRows];  // by tile's parity; gain by tile % 4
     __shared__ int unit_exp[2];
+    __shared__ float col_sum[W ? 2 : 1][2][4][kTileKeys];  // by tile's parity, alternating
     __shared__ uint32_t tmem_slot, abort_flag;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
 
     const KvAttnCall& a = P.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int h = blockIdx.x % a.c.H, gt = P.tiles - 1 - blockIdx.x / a.c.H, split = blockIdx.y, G = a.G;
+    const int h = blockIdx.x % a.c.H, gt = (W ? P.tile0 : 0) + P.tiles - 1 - blockIdx.x / a.c.H, split = blockIdx.y, G = a.G;
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < 2; i++) {
@@ -137,6 +149,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             mbar_init(&bar_v_full[i], 128);
             mbar_init(&bar_v_empty[i], 1);
             mbar_init(&bar_raw[i], 4);
+            mbar_init(&bar_raw_empty[i], 128);
+            mbar_init(&bar_w[i], 128);
             mbar_init(&bar_s[i], 1);
             mbar_init(&bar_m[i], 128);
             mbar_init(&bar_p[i][0], 128);
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     griddep_launch_dependents();
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
         const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-        if (blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
+        if (!W && blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
         return prompt_tiles(a, s);
     });
     tc_fence_after();
@@ -251,14 +265,68 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         mbar_arrive(&bar_q);
         const int lim = p < pairs ? kv_limit(a, q, p / G) : 0;
         const uint32_t ts = lanes + kColS + X * 128;
-        float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
-        int E = -100;                  // P_i holds p (dv / 2^(E - 15))
         // lane j < 4: the scales of key tile i's block j; blocks past the end hold anything
         auto fetch = [&](int i) {
             const int b = (t0 + i) * (kTileKeys / kKvBlock) + lane;
             return lane < 4 && i < n && b * kKvBlock < q.len ? scales[b] : make_float2(0.f, 0.f);
         };
         float2 next = fetch(X);
+        if constexpr (W) {
+            float* const dst = P.wpart + ((int64_t)(gt - P.tile0) * a.c.H + h) * P.wkeys;
+            const float lse = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : INFINITY;
+            for (int i = X; i < n; i += 2) {
+                const int key0 = (t0 + i) * kTileKeys;
+                const float2 sc = next;
+                next = fetch(i + 2);
+                if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) break;
+                tc_fence_after();
+                const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
+                float* const cols = col_sum[X][(i >> 1) & 1][warp & 3];
+                auto add_up = [&](auto masked) {
+#pragma unroll 1
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t r[32];
+                        float w[32];
+                        tmem_ld32(ts + 32 * j, r);
+                        const float k = coef * __shfl_sync(0xffffffffu, sc.x, j);
+                        tmem_ld_wait_dep(r);
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float p0 = -lse, p1 = -lse;
+                            ffma2(p0, p1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k, k);
+                            w[c] = kv_ex2(p0);
+                            w[c + 1] = kv_ex2(p1);
+                            if (decltype(masked)::value) {
+                                const int t = key0 + 32 * j + c;
+                                if (t >= lim) w[c] = 0.f;
+                                if (t + 1 >= lim) w[c + 1] = 0.f;
+                            }
+                        }
+                        // each step adds two rows and halves the columns that a lane holds
+#pragma unroll
+                        for (int half = 16; half; half >>= 1)
+#pragma unroll
+                            for (int c = 0; c < half; c++) {
+                                const bool up = lane & half;
+                                const float give = up ? w[c] : w[c + half];
+                                const float keep = up ? w[c + half] : w[c];
+                                w[c] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+                            }
+                        cols[32 * j + lane] = w[0];
+                    }
+                };
+                if (full) add_up(std::false_type{});
+                else add_up(std::true_type{});
+                tc_fence_before();
+                mbar_arrive(&bar_p[X][0]);
+                mbar_arrive(&bar_w[X]);
+                if (!mbar_wait(&bar_w[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutScaleFull)) break;
+                const float(&c4)[4][kTileKeys] = col_sum[X][(i >> 1) & 1];
+                dst[key0 + row] = (c4[0][row] + c4[1][row]) + (c4[2][row] + c4[3][row]);
+            }
+        } else {
+        float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
+        int E = -100;                  // P_i holds p (dv / 2^(E - 15))
         for (int i = X; i < n; i += 2) {
             const int key0 = (t0 + i) * kTileKeys;
             const float2 sc = next;
@@ -361,8 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         row_sum[X][row] = l;
         if (row == 0) unit_exp[X] = E;
         named_bar_sync(1, 384);
+        }
     } else if (warp < 12) {
         regs_inc<kRegsSum>();
+        if constexpr (!W) {
         const uint32_t to = lanes + kColO;
         float o[D];
         bool ok = true;
@@ -421,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 for (int d = 0; d < D; d++) dst[d] = o[d] * scale * back;
             }
         }
+        }
     } else if (warp < 16) {
         regs_dec<kRegsConvert>();
         const int cw = warp - 12, qn = lane / 4, qc = lane % 4;
@@ -473,8 +544,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             fence_proxy_async_smem();
             mbar_arrive(&bar_k_full[B]);
             if (i == 0 && !mbar_wait(&bar_q, 0, &abort_flag, status, kDevTimeoutEmpty)) break;  // the queries have left V's place and K's second
-            if (i > 1 && !mbar_wait(&bar_v_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
-            {
+            if (!W && i > 1 && !mbar_wait(&bar_v_empty[B], ph, &abort_flag, status, kDevTimeoutEmpty)) break;
+            if constexpr (!W) {
                 const uint32_t rv = raw + bv * REC + 32 * D;
                 const uint32_t vb = sb + M::V + B * M::V_TILE + cw / 2 * M::V_PANEL + qn * 128 + (((4 * (bv & 1) + qc) ^ qn) << 4);
                 constexpr int VG = D / 16 % 4 == 0 ? 4 : 5;
@@ -491,11 +562,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                     }
                 }
             }
-            fence_proxy_async_smem();
-            mbar_arrive(&bar_v_full[B]);
-            named_bar_sync(2, 128);  // the tile's codes are read by all four warps
+            if (!W) {
+                fence_proxy_async_smem();
+                mbar_arrive(&bar_v_full[B]);
+            }
+            mbar_arrive(&bar_raw_empty[B]);
             if (i + 2 < n) {
-                if (lane == 0) copy_codes(i + 2, cw);
+                if (lane == 0) {  // all four warps have read the tile's codes
+                    if (!mbar_wait(&bar_raw_empty[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutEmpty)) break;
+                    copy_codes(i + 2, cw);
+                }
                 issued = i + 3;
             }
         }
@@ -528,6 +604,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             };
             auto pv = [&](int i, auto parity) {
                 constexpr int B = decltype(parity)::value;
+                if constexpr (W)  // the softmax warps are done with S_i
+                    return mbar_wait(&bar_p[B][0], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty);
                 if (!mbar_wait(&bar_v_full[B], (i >> 1) & 1, &abort_flag, status, kDevTimeoutFull)) return false;
                 if (i > 0 && !mbar_wait(&bar_o_empty, (i - 1) & 1, &abort_flag, status, kDevTimeoutTmemEmpty)) return false;
 #pragma unroll
@@ -615,9 +693,34 @@ __global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptP
     if (P.lse && lane == 0) P.lse[row * a.heads + head] = none ? INFINITY : m + log2f(l);
 }
 
+// weights_out = base + the sums of the batch's tiles, in their order
+__global__ void __launch_bounds__(128) k_kv_weight_sum(const __grid_constant__ PromptParams P, const float* base)
+{
+    __shared__ int sum[kKvMaxSequences + 1];
+    __shared__ int warp_sums[32];
+    const KvAttnCall& a = P.a;
+    griddep_wait();
+    griddep_launch_dependents();
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles(a, s); });
+    const int s = blockIdx.z, h = blockIdx.y;
+    const int64_t key = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    if (key >= q.len) return;
+    const int g0 = max(sum[s], P.tile0), g1 = min(sum[s + 1], P.tile0 + P.tiles);
+    float w = 0.f;
+#pragma unroll 4
+    for (int g = g0; g < g1; g++) {
+        const int last = min(q.n * a.G, (g - sum[s] + 1) * kTileRows) - 1;
+        if (key < kv_limit(a, q, last / a.G)) w += P.wpart[((int64_t)(g - P.tile0) * a.c.H + h) * P.wkeys + key];
+    }
+    const int64_t at = ((int64_t)s * a.c.H + h) * a.c.cap + key;
+    a.weights_out[at] = (base ? base[at] : 0.f) + w;
+}
+
 struct PromptPlan {
     int tiles, splits;
-    size_t part_bytes;
+    int64_t wkeys, wtiles;  // weights: keys per partial row, pair tiles per pass
+    size_t part_bytes;      // (the weights' sums take the place of the split parts)
 };
 
 PromptPlan plan_prompt(const KvAttnCall& a, int num_sms)
@@ -630,7 +733,35 @@ PromptPlan plan_prompt(const KvAttnCall& a, int num_sms)
     const int64_t key_tiles = (a.c.cap + kTileKeys - 1) / kTileKeys;
     p.splits = (int)std::max<int64_t>(1, std::min(key_tiles, num_sms / (most * a.c.H)));
     p.part_bytes = p.splits > 1 ? (size_t)p.splits * p.tiles * a.c.H * kTileRows * (a.c.D + 2) * sizeof(float) : 0;
+    if (a.weights_out) {
+        // as many tiles at a time as 256 MB of partial sums hold
+        p.wkeys = key_tiles * kTileKeys;
+        const int64_t per = p.wkeys * a.c.H * (int64_t)sizeof(float);
+        p.wtiles = std::max<int64_t>(1, std::min<int64_t>(p.tiles, ((int64_t)256 << 20) / per));
+        p.part_bytes = std::max(p.part_bytes, (size_t)(p.wtiles * per));
+    }
     return p;
+}
+
+template <int D>
+cudaError_t launch_weights(PromptParams P, const PromptPlan& p, int num_sms, cudaStream_t s, int* launches)
+{
+    constexpr int smem = PromptSmem<D>::BYTES;
+    static std::atomic<uint32_t> done{0};
+    cudaError_t e = allow_smem(k_kv_prompt<D, true>, smem, done);
+    P.wpart = P.part;
+    P.wkeys = p.wkeys;
+    for (int64_t t = 0; t < p.tiles && e == cudaSuccess; t += p.wtiles) {
+        P.tile0 = (int)t;
+        P.tiles = (int)std::min(p.wtiles, p.tiles - t);
+        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>(p.wkeys / kTileKeys, num_sms / ((int64_t)P.tiles * P.a.c.H)));
+        e = launch_pdl(k_kv_prompt<D, true>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
+        if (e != cudaSuccess) break;
+        e = launch_pdl(k_kv_weight_sum, dim3((unsigned)((P.a.c.cap + 127) / 128), (unsigned)P.a.c.H, (unsigned)P.a.c.S), dim3(128), 0, s, P,
+                       t ? (const float*)P.a.weights_out : P.a.weights);
+        *launches += 2;
+    }
+    return e;
 }
 
 template <int D>
@@ -638,9 +769,9 @@ cudaError_t launch_d(const PromptParams& P, cudaStream_t s)
 {
     constexpr int smem = PromptSmem<D>::BYTES;
     static std::atomic<uint32_t> done{0};
-    cudaError_t e = allow_smem(k_kv_prompt<D>, smem, done);
+    cudaError_t e = allow_smem(k_kv_prompt<D, false>, smem, done);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(k_kv_prompt<D>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
+    e = launch_pdl(k_kv_prompt<D, false>, dim3((unsigned)(P.tiles * P.a.c.H), (unsigned)P.splits), dim3(kThreads), smem, s, P);
     if (e != cudaSuccess || P.splits == 1) return e;
     const int64_t pairs = std::min<int64_t>(kTileRows, P.a.max_rows * P.a.G);
     return launch_pdl(k_kv_join<D>, dim3((unsigned)P.tiles, (unsigned)P.a.c.H, (unsigned)((pairs + 7) / 8)), dim3(256), 0, s, P);
@@ -660,10 +791,15 @@ cudaError_t launch_kv_prompt(const KvAttnCall& a, float* part, float* lse, int n
     P.tiles = p.tiles;
     P.splits = p.splits;
     *launches = p.splits > 1 ? 2 : 1;
+    auto run = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        const cudaError_t e = launch_d<D>(P, s);
+        return e != cudaSuccess || !a.weights_out ? e : launch_weights<D>(P, p, num_sms, s, launches);
+    };
     switch (a.c.D) {
-    case 64: return launch_d<64>(P, s);
-    case 80: return launch_d<80>(P, s);
-    case 128: return launch_d<128>(P, s);
+    case 64: return run(std::integral_constant<int, 64>{});
+    case 80: return run(std::integral_constant<int, 80>{});
+    case 128: return run(std::integral_constant<int, 128>{});
     default: return cudaErrorInvalidValue;
     }
 }
