@@ -21,43 +21,74 @@ namespace {
 
 constexpr float kKvTiny = 3.009265538105056e-36f;  // 2^-118: blocks below it are stored as zeros (1 / d stays finite)
 
-// Largest magnitudes of the CTA's K and V values; not finite: +inf.
-__device__ __forceinline__ float kv_mag(float m, float x)
+// max(m, |a|, |b|), NaN if one of them is.
+__device__ __forceinline__ float kv_mag(float m, float a, float b)
 {
-    const float a = fabsf(x);
-    return a <= FLT_MAX ? fmaxf(m, a) : INFINITY;
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
 }
+// Largest magnitudes of the CTA's K and V values.
 __device__ __forceinline__ float2 kv_block_max(float mk, float mv, float2* red)
 {
 #pragma unroll
     for (int off = 16; off; off >>= 1) {
-        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, off));
-        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, off));
+        mk = kv_mag(mk, __shfl_xor_sync(0xffffffffu, mk, off), 0.f);
+        mv = kv_mag(mv, __shfl_xor_sync(0xffffffffu, mv, off), 0.f);
     }
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(mk, mv);
     __syncthreads();
     for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
-        mk = fmaxf(mk, red[w].x);
-        mv = fmaxf(mv, red[w].y);
+        mk = kv_mag(mk, red[w].x, 0.f);
+        mv = kv_mag(mv, red[w].y, 0.f);
     }
     return make_float2(mk, mv);
 }
 __device__ __forceinline__ float kv_scale(float a)
 {
-    if (a == INFINITY) return __int_as_float(0x7fffffff);
+    if (!(a <= FLT_MAX)) return __int_as_float(0x7fffffff);
     return a < kKvTiny ? 0.f : __fdiv_rn(a, 127.f);
 }
 
-// Code byte of x under scale d (inv = 1 / d rounded): the integer nearest to
-// x / d, ties to even.  rint(x * inv) is within one of it, and r = x - q d is
-// exact (|r| < 2 d on the grid of d's last place), so comparing 2 |r| with d
-// settles it.
-__device__ __forceinline__ uint32_t kv_code(float x, float d, float inv)
+// 16 code bytes under scale d (inv = 1 / d rounded): the integers nearest to
+// x / d, ties to even, plus 128.  x * inv + 1.5 * 2^23 + 128, rounded once,
+// has the code byte in its low bits and is within one of the right integer;
+// r = x - q d is exact (|r| < 2 d on the grid of d's last place), so 2 |r| < d
+// says that it is right.  Where a value of the thread lies so near to a border
+// that this fails, all are settled by comparison.
+__device__ __forceinline__ void kv_codes(const float (&x)[16], float d, float inv, uint32_t (&w)[4])
 {
-    float q = rintf(__fmul_rn(x, inv));
-    const float r = __fmaf_rn(-q, d, x), e = 2.f * fabsf(r);
-    if (e > d || (e == d && ((int)q & 1))) q += copysignf(1.f, r);
-    return (uint32_t)((int)q + 128) & 255u;
+    constexpr float kMagic = 12582912.f + 128.f;
+    if (!(d > 0.f)) {
+        w[0] = w[1] = w[2] = w[3] = 0x80808080u;
+        return;
+    }
+    uint32_t c[16];
+    const float half = 0.5f * d;
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float m = __fmaf_rn(x[i], inv, kMagic);
+        c[i] = __float_as_uint(m);
+        near |= fabsf(__fmaf_rn(-(m - kMagic), d, x[i])) >= half;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float q = __uint_as_float(c[i]) - kMagic;
+            const float r = __fmaf_rn(-q, d, x[i]), e = fabsf(r);
+            if (e > half || (e == half && (c[i] & 1u))) q += copysignf(1.f, r);
+            c[i] = __float_as_uint(q + kMagic);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+}
+// Byte `sel` (0..7) of (lo, hi) as the number it stands for.
+__device__ __forceinline__ float kv_number(uint32_t lo, uint32_t hi, uint32_t sel)
+{
+    return __uint_as_float(__byte_perm(__byte_perm(lo, hi, sel), 0x4b000000u, 0x7440)) - (8388608.f + 128.f);
 }
 
 // Quantize and store a block from registers: xk = 16 channels (16 * kc ..) of
@@ -70,33 +101,23 @@ __device__ __forceinline__ void kv_store_block(const KvView& c, int64_t sh, int 
     const int tid = threadIdx.x, kt = tid / (D / 16), kc = tid % (D / 16), vd = tid % D, vt = tid / D;
     float mk = 0.f, mv = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        mk = kv_mag(mk, xk[i]);
-        mv = kv_mag(mv, xv[i]);
+    for (int i = 0; i < 16; i += 2) {
+        mk = kv_mag(mk, xk[i], xk[i + 1]);
+        mv = kv_mag(mv, xv[i], xv[i + 1]);
     }
     const float2 m = kv_block_max(mk, mv, red);
     const float dk = kv_scale(m.x), dv = kv_scale(m.y);
     const float ik = dk > 0.f ? __fdiv_rn(1.f, dk) : 0.f, iv = dv > 0.f ? __fdiv_rn(1.f, dv) : 0.f;
     uint8_t* rec = c.codes + (sh * c.nb + b) * kv_record_bytes(D);
     uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[i] |= (dk > 0.f ? kv_code(xk[4 * i + j], dk, ik) : 128u) << (8 * j);
-    }
+    kv_codes(xk, dk, ik, w);
     if (D % 64 != 0 && kc >= D / 64 * 4) {
 #pragma unroll
         for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t*>(rec + kv_k_offset<D>(kt, 16 * kc + 4 * i)) = w[i];
     } else {
         *reinterpret_cast<uint4*>(rec + kv_k_offset<D>(kt, 16 * kc)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[i] |= (dv > 0.f ? kv_code(xv[4 * i + j], dv, iv) : 128u) << (8 * j);
-    }
+    kv_codes(xv, dv, iv, w);
     *reinterpret_cast<uint2*>(rec + kv_v_offset<D>(16 * vt, vd)) = make_uint2(w[0], w[1]);
     *reinterpret_cast<uint2*>(rec + kv_v_offset<D>(16 * vt + 8, vd)) = make_uint2(w[2], w[3]);
     if (tid == 0) c.scales[sh * c.nb + b] = make_float2(dk, dv);
@@ -123,8 +144,8 @@ __device__ __forceinline__ void kv_values(const KvView& c, int64_t sh, int b, fl
     const uint32_t z[4] = {a.x, a.y, e.x, e.y};
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        xk[i] = __fmul_rn((float)((int)((w[i / 4] >> (8 * (i % 4))) & 255u) - 128), d.x);
-        xv[i] = __fmul_rn((float)((int)((z[i / 4] >> (8 * (i % 4))) & 255u) - 128), d.y);
+        xk[i] = __fmul_rn(kv_number(w[i / 4], 0, i % 4), d.x);
+        xv[i] = __fmul_rn(kv_number(z[i / 4], 0, i % 4), d.y);
     }
 }
 
@@ -166,7 +187,7 @@ __device__ __forceinline__ int kv_touched(const KvView& c, int len, int n)
 }
 
 template <int D>
-__global__ void __launch_bounds__(2 * D)
+__global__ void __launch_bounds__(2 * D, 4)
     k_kv_append(const __grid_constant__ KvView c, const float* k, int64_t ldk, const float* v, int64_t ldv,
                 int64_t rows, const int32_t* starts, int veck, uint32_t* status)
 {
@@ -327,13 +348,22 @@ __device__ __forceinline__ uint32_t kv_order(float w)
 // and the keep - recent largest weights of the others.  The border value is
 // found by three histogram passes (11, 11 and 10 bits of the ordered
 // integer), then one pass in index order writes what lies above it and the
-// first ties.  Integer counts only, so the result is exact.
-constexpr int SEL_THREADS = 1024, SEL_ITEMS = 4, SEL_BINS = 2048;
+// first ties.  Integer counts only, so the result is exact.  The integers stay
+// in shared memory from the first pass on, as many as fit.
+constexpr int SEL_THREADS = 1024, SEL_BINS = 2048, SEL_CACHE = 50 * 1024;
+
+// Sum of x[0 .. warp - 1] (warp <= 32 values), by every warp for itself.
+__device__ __forceinline__ uint32_t sel_before(const uint32_t* x, int warp, int lane)
+{
+    uint32_t v = lane < warp ? x[lane] : 0u;
+    return __reduce_add_sync(0xffffffffu, v);
+}
 
 __global__ void __launch_bounds__(SEL_THREADS)
     k_kv_select(const __grid_constant__ KvView c, const __grid_constant__ KvView dst, const float* weights, int keep,
                 int recent, float* weights_out, int32_t* kept)
 {
+    extern __shared__ uint32_t keys[];  // [min(old, SEL_CACHE)]
     __shared__ uint32_t bins[SEL_BINS];
     __shared__ uint32_t warp_sums[32], found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.x, s = blockIdx.y;
@@ -360,10 +390,28 @@ __global__ void __launch_bounds__(SEL_THREADS)
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
             for (int i = tid; i < SEL_BINS; i += SEL_THREADS) bins[i] = 0;
             __syncthreads();
-            for (int i = tid; i < old; i += SEL_THREADS) {
-                const uint32_t u = kv_order(w[i]);
+            auto count_in = [&](uint32_t u) {
                 if ((u & mask) == border) atomicAdd(&bins[(u >> shift) & (width - 1)], 1u);
+            };
+            const int cached = min(old, SEL_CACHE);
+            if (pass == 0) {
+                for (int i0 = tid; i0 < cached; i0 += 8 * SEL_THREADS) {
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = i0 + k * SEL_THREADS < cached ? w[i0 + k * SEL_THREADS] : 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (i0 + k * SEL_THREADS < cached) {
+                            const uint32_t u = kv_order(x[k]);
+                            keys[i0 + k * SEL_THREADS] = u;
+                            count_in(u);
+                        }
+                }
+            } else {
+#pragma unroll 4
+                for (int i = tid; i < cached; i += SEL_THREADS) count_in(keys[i]);
             }
+            for (int i = cached + tid; i < old; i += SEL_THREADS) count_in(kv_order(w[i]));
             __syncthreads();
             // the bin that holds the want-th largest: counts from the top, two bins per thread
             const int hi = SEL_BINS - 1 - 2 * tid;
@@ -376,7 +424,7 @@ __global__ void __launch_bounds__(SEL_THREADS)
             }
             if (lane == 31) warp_sums[warp] = v;
             __syncthreads();
-            for (int i = 0; i < warp; i++) v += warp_sums[i];
+            v += sel_before(warp_sums, warp, lane);
             const uint32_t before = v - a - b;
             if (before < want && want <= before + a) {
                 found[0] = (uint32_t)hi;
@@ -393,107 +441,110 @@ __global__ void __launch_bounds__(SEL_THREADS)
         }
         if (count > rec) ties = want;
     }
-    // one pass in order: kept tokens so far, ties so far
-    uint32_t sel = 0, tied = 0;
-    for (int base = 0; base < len; base += SEL_THREADS * SEL_ITEMS) {
-        uint32_t above[SEL_ITEMS], equal[SEL_ITEMS], mine = 0;  // counts: above in the low half, equal in the high half
-        float x[SEL_ITEMS];
-#pragma unroll
-        for (int i = 0; i < SEL_ITEMS; i++) {
-            const int t = base + tid * SEL_ITEMS + i;
-            x[i] = t < len ? w[t] : 0.f;
-            const uint32_t u = kv_order(x[i]);
-            above[i] = t < len && (t >= old || u > border);
-            equal[i] = t < old && u == border;
-            mine += above[i] | equal[i] << 16;
+    // In order: a warp takes a stretch of the tokens, counts what it keeps and its ties, and writes from where the warps
+    // before it end.
+    const int stretch = (len + SEL_THREADS - 1) / SEL_THREADS * 32;
+    const int first = min(len, warp * stretch), last = min(len, first + stretch);
+    const uint32_t below = (1u << lane) - 1u;
+    const bool keyed = len > keep && count > rec;  // keys[] holds the first tokens' integers
+    const int cached = keyed ? min(old, SEL_CACHE) : 0;
+    auto look = [&](int t, uint32_t& above, uint32_t& equal) {
+        const uint32_t u = t < cached ? keys[t] : t < old ? kv_order(w[t]) : 0u;
+        above = __ballot_sync(0xffffffffu, t < last && (t >= old || u > border));
+        equal = __ballot_sync(0xffffffffu, t < last && t < old && u == border);
+    };
+    uint32_t na = 0, ne = 0;
+    for (int t0 = first; t0 < last; t0 += 32) {
+        uint32_t above, equal;
+        look(t0 + lane, above, equal);
+        na += __popc(above);
+        ne += __popc(equal);
+    }
+    __syncthreads();
+    if (lane == 0) warp_sums[warp] = na, bins[warp] = ne;
+    __syncthreads();
+    na = sel_before(warp_sums, warp, lane);
+    ne = sel_before(bins, warp, lane);
+    for (int t0 = first; t0 < last; t0 += 32) {
+        uint32_t above, equal;
+        look(t0 + lane, above, equal);
+        const uint32_t a = na + __popc(above & below), e = ne + __popc(equal & below);
+        if ((above >> lane & 1u) || ((equal >> lane & 1u) && e < ties)) {
+            const uint32_t at = a + min(e, ties);
+            kept[at] = t0 + lane;
+            if (wo) wo[at] = w[t0 + lane];
         }
-        uint32_t v = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, v, off);
-            if (lane >= off) v += y;
-        }
-        if (lane == 31) warp_sums[warp] = v;
-        __syncthreads();
-        uint32_t before = v - mine, all = 0;
-        for (int i = 0; i < 32; i++) {
-            const uint32_t y = warp_sums[i];
-            if (i < warp) before += y;
-            all += y;
-        }
-        uint32_t na = sel + (before & 0xffffu), ne = tied + (before >> 16);
-#pragma unroll
-        for (int i = 0; i < SEL_ITEMS; i++) {
-            const bool take = above[i] || (equal[i] && ne < ties);
-            if (take) {
-                const uint32_t at = na + min(ne, ties);
-                kept[at] = base + tid * SEL_ITEMS + i;
-                if (wo) wo[at] = x[i];
-            }
-            na += above[i];
-            ne += equal[i];
-        }
-        sel += all & 0xffffu;
-        tied += all >> 16;
-        __syncthreads();
+        na += __popc(above);
+        ne += __popc(equal);
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(2 * D) k_kv_compact(const __grid_constant__ KvView c, const __grid_constant__ KvView dst,
+// NB destination blocks per CTA: their tokens' places and scales are looked up
+// at once.  All loads of a block are issued before the first is used, and four
+// CTAs share an SM: the kernel waits for memory (8 x 32768 tokens to 8191, 4
+// heads of 128: 107 us with the selection, 155 us at two CTAs per SM).
+template <int D, int NB>
+__global__ void __launch_bounds__(2 * D, 4) k_kv_compact(const __grid_constant__ KvView c, const __grid_constant__ KvView dst,
                                                       const int32_t* kept, int keep)
 {
-    __shared__ float2 red[2 * D / 32];
-    __shared__ int from[kKvBlock];
-    __shared__ float2 scale[kKvBlock];
-    const int tid = threadIdx.x, b = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
+    __shared__ float2 red[NB][2 * D / 32];
+    __shared__ uint32_t from[NB * kKvBlock];
+    __shared__ float2 scale[NB * kKvBlock];
+    const int tid = threadIdx.x, h = blockIdx.y, s = blockIdx.z, b0 = blockIdx.x * NB;
     griddep_wait();
     griddep_launch_dependents();
     const int count = min(c.lens[s], keep);
-    if (b * kKvBlock >= count) return;
     const int64_t sh = (int64_t)s * c.H + h;
-    if (tid < kKvBlock) {
-        const int i = b * kKvBlock + tid;
-        const int t = i < count ? kept[sh * keep + i] : -1;
+    const int total = min(NB * kKvBlock, count - b0 * kKvBlock);  // tokens of these blocks
+    if (total <= 0) return;
+    if (tid < NB * kKvBlock) {
+        const uint32_t t = kept[sh * keep + b0 * kKvBlock + min(tid, total - 1)];  // (absent ones: a token's bytes all the same)
         from[tid] = t;
-        if (t >= 0) scale[tid] = c.scales[sh * c.nb + t / kKvBlock];
+        scale[tid] = c.scales[sh * c.nb + t / kKvBlock];
     }
     __syncthreads();
     const int kt = tid / (D / 16), kc = tid % (D / 16), vd = tid % D, vt = tid / D;
     const uint8_t* base = c.codes + sh * c.nb * kv_record_bytes(D);
-    float xk[16], xv[16];
+#pragma unroll 1
+    for (int u = 0; u < NB && u * kKvBlock < total; u++) {
+        const int here = min(kKvBlock, total - u * kKvBlock);
+        const uint32_t* ft = from + u * kKvBlock;
+        const float2* sc = scale + u * kKvBlock;
+        uint2 g[16];  // V: the group of eight tokens that holds the token
 #pragma unroll
-    for (int i = 0; i < 16; i++) xk[i] = 0.f;
-    if (from[kt] >= 0) {
-        const int t = from[kt];
-        const uint8_t* rec = base + (int64_t)(t / kKvBlock) * kv_record_bytes(D);
+        for (int i = 0; i < 16; i++) {
+            const uint32_t t = ft[16 * vt + i];
+            g[i] = *reinterpret_cast<const uint2*>(base + (int64_t)(t / kKvBlock) * kv_record_bytes(D) + kv_v_offset<D>(t % kKvBlock & ~7u, vd));
+        }
         uint32_t w[4];
-        if (D % 64 != 0 && kc >= D / 64 * 4) {
+        {
+            const uint32_t t = ft[kt];
+            const uint8_t* rec = base + (int64_t)(t / kKvBlock) * kv_record_bytes(D);
+            if (D % 64 != 0 && kc >= D / 64 * 4) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint32_t*>(rec + kv_k_offset<D>(t % kKvBlock, 16 * kc + 4 * i));
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(rec + kv_k_offset<D>(t % kKvBlock, 16 * kc));
-            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint32_t*>(rec + kv_k_offset<D>(t % kKvBlock, 16 * kc + 4 * i));
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4*>(rec + kv_k_offset<D>(t % kKvBlock, 16 * kc));
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            }
         }
+        float xk[16], xv[16];
+        const float sk = sc[kt].x;
 #pragma unroll
-        for (int i = 0; i < 16; i++) xk[i] = __fmul_rn((float)((int)((w[i / 4] >> (8 * (i % 4))) & 255u) - 128), scale[kt].x);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int t = from[16 * vt + i];
-        xv[i] = 0.f;
-        if (t >= 0) {
-            const uint8_t q = base[(int64_t)(t / kKvBlock) * kv_record_bytes(D) + kv_v_offset<D>(t % kKvBlock, vd)];
-            xv[i] = __fmul_rn((float)((int)q - 128), scale[16 * vt + i].y);
+        for (int i = 0; i < 16; i++) {
+            const uint32_t t = ft[16 * vt + i];
+            xk[i] = kt < here ? __fmul_rn(kv_number(w[i / 4], 0, i % 4), sk) : 0.f;
+            xv[i] = 16 * vt + i < here ? __fmul_rn(kv_number(g[i].x, g[i].y, t & 7), sc[16 * vt + i].y) : 0.f;
         }
-    }
-    if (b == (count - 1) / kKvBlock) {
-        st16(kv_tail(dst, s, 0, h, 0) + kt * D + 16 * kc, xk, true);
-        float* tv = kv_tail(dst, s, 0, h, 1);
+        const int b = b0 + u;
+        if (b == (count - 1) / kKvBlock) {
+            st16(kv_tail(dst, s, 0, h, 0) + kt * D + 16 * kc, xk, true);
+            float* tv = kv_tail(dst, s, 0, h, 1);
 #pragma unroll
-        for (int i = 0; i < 16; i++) tv[(16 * vt + i) * D + vd] = xv[i];
+            for (int i = 0; i < 16; i++) tv[(16 * vt + i) * D + vd] = xv[i];
+        }
+        kv_store_block<D>(dst, sh, b, xk, xv, red[u]);
     }
-    kv_store_block<D>(dst, sh, b, xk, xv, red);
 }
 
 template <typename F>
@@ -573,14 +624,21 @@ cudaError_t launch_kv_read(const KvView& c, const int32_t* first, int64_t count,
 cudaError_t launch_kv_evict(const KvView& src, const KvView& dst, const float* weights, int64_t keep, int64_t recent,
                             float* weights_out, int32_t* kept, cudaStream_t s)
 {
-    cudaError_t e = launch_pdl(k_kv_select, dim3((unsigned)src.H, (unsigned)src.S), dim3(SEL_THREADS), 0, s, src, dst, weights,
-                               (int)keep, (int)recent, weights_out, kept);
+    static std::atomic<uint32_t> done{0};
+    cudaError_t e = allow_smem(k_kv_select, SEL_CACHE * 4, done);
+    if (e != cudaSuccess) return e;
+    const size_t smem = (size_t)std::min<int64_t>(src.cap, SEL_CACHE) * 4;
+    e = launch_pdl(k_kv_select, dim3((unsigned)src.H, (unsigned)src.S), dim3(SEL_THREADS), smem, s, src, dst, weights, (int)keep,
+                   (int)recent, weights_out, kept);
     if (e != cudaSuccess) return e;
     const int64_t blocks = (std::min(keep, (int64_t)src.cap) + kKvBlock - 1) / kKvBlock;
     return by_dim(src.D, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return launch_pdl(k_kv_compact<D>, dim3((unsigned)blocks, (unsigned)src.H, (unsigned)src.S), dim3(2 * D), 0, s, src, dst, kept,
-                          (int)keep);
+        // four blocks per CTA once there is work for every SM many times over
+        const auto kernel = blocks * src.H * src.S >= 8192 ? k_kv_compact<D, 4> : k_kv_compact<D, 1>;
+        const int per = kernel == k_kv_compact<D, 4> ? 4 : 1;
+        return launch_pdl(kernel, dim3((unsigned)((blocks + per - 1) / per), (unsigned)src.H, (unsigned)src.S), dim3(2 * D), 0, s, src, dst,
+                          (const int32_t*)kept, (int)keep);
     });
 }
 
