@@ -32,7 +32,7 @@ constexpr int kMinRun = 4;               // fewest blocks worth a CTA: one per w
 // D += A (16 x 16, row) * B (16 x 8, column), fp16 in, fp32 out
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -52,7 +52,44 @@ __device__ __forceinline__ int kv_attn_blocks(const KvAttnCall& a, int s)
     if (q.n <= 0 || q.n > a.max_rows) return 0;
     return max(1, (q.len + kKvBlock - 1) / kKvBlock);
 }
-__device__ __forceinline__ int kv_run_length(int total, int runs) { return max(kMinRun, (total + runs - 1) / runs); }
+// How the CTAs divide the (sequence, head)s' blocks.  Taking up another
+// (sequence, head) costs a CTA about as much as kSegmentCost blocks (queries
+// to fetch and split, warps to join), so each is cut into equal parts of its
+// own, a part per CTA, as many as the CTAs allow: with T blocks, N CTAs and n
+// (sequence, head)s, parts of T / (N - n) blocks always fit.  Where that makes
+// them longer than an equal share T / N by more than kSegmentCost, CTA i takes
+// blocks [i run, (i + 1) run) of the flattened list instead, whatever they
+// belong to.
+constexpr int kSegmentCost = 10;
+struct KvDivision {
+    int part;  // most blocks of a part, sum[s]: parts before sequence s; 0: the flattened list
+    int run;   // flattened: blocks per CTA, sum[s]: blocks before sequence s
+};
+__device__ __forceinline__ KvDivision kv_divide(const KvAttnCall& a, int runs, int* sum, int* warp_sums)
+{
+    const int S = a.c.S, H = a.c.H, n = S * H;
+    auto decide = [&](int total) {
+        KvDivision d;
+        d.run = max(kMinRun, (total + runs - 1) / runs);
+        d.part = n < runs ? max(kMinRun, (total + runs - n - 1) / (runs - n)) : 0;
+        if (d.part - d.run > kSegmentCost) d.part = 0;
+        return d;
+    };
+    if (S == 1) {
+        const int nb = kv_attn_blocks(a, 0);
+        const KvDivision d = decide(nb * H);
+        if (threadIdx.x == 0) sum[0] = 0, sum[1] = (d.part ? (nb + d.part - 1) / d.part : nb) * H;
+        __syncthreads();
+        return d;
+    }
+    kv_prefix(S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * H; });
+    const KvDivision d = decide(sum[S]);
+    if (d.part) {
+        __syncthreads();  // everyone has read the total
+        kv_prefix(S, sum, warp_sums, [&](int s) { return (kv_attn_blocks(a, s) + d.part - 1) / d.part * H; });
+    }
+    return d;
+}
 
 // One warp's A fragments of up to PT pairs' queries: PT = 8 packs hi into
 // rows 0-7 and lo into rows 8-15 of one fragment, PT = 16 keeps two.
@@ -128,15 +165,18 @@ __device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_
     for (int nt = 0; nt < 4; nt++)
 #pragma unroll
         for (int i = 0; i < 4; i++) s[nt][i] = 0.f;
+    // the four token groups' sums are independent: their products take turns, so that none waits for the one before it
 #pragma unroll
     for (int j = 0; j < J; j++) {
+        uint4 w[4];
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) {
-            const uint4 w = *reinterpret_cast<const uint4*>(rec + ((nt * J + j) * 32 + lane) * 16);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        for (int nt = 0; nt < 4; nt++) w[nt] = *reinterpret_cast<const uint4*>(rec + ((nt * J + j) * 32 + lane) * 16);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t b0 = kv_half2_lo(ww[k]), b1 = kv_half2_hi(ww[k]);
+        for (int k = 0; k < 4; k++) {
+#pragma unroll
+            for (int nt = 0; nt < 4; nt++) {
+                const uint32_t ww = k == 0 ? w[nt].x : k == 1 ? w[nt].y : k == 2 ? w[nt].z : w[nt].w;
+                const uint32_t b0 = kv_half2_lo(ww), b1 = kv_half2_hi(ww);
                 mma16816(s[nt], q.hi[4 * j + k], b0, b1);
                 if (PT == 16) mma16816(s[nt], q.lo[4 * j + k], b0, b1);
             }
@@ -165,7 +205,7 @@ __device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_
         }
 }
 
-constexpr int kAttnStages = 3;  // blocks in flight per warp
+constexpr int kAttnStages = 2;  // blocks in flight per warp
 template <int D>
 constexpr size_t attn_smem_bytes() { return (size_t)AW * kAttnStages * kv_record_bytes(D); }
 
@@ -192,12 +232,13 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
     }
     griddep_wait();
     griddep_launch_dependents();
-    kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
-        const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-        if (blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
-        return kv_attn_blocks(a, s) * a.c.H;
-    });
-    const int total = sum[a.c.S], run = kv_run_length(total, P.runs);
+    const KvDivision dv = kv_divide(a, P.runs, sum, warp_sums);
+    const int total = sum[a.c.S], run = dv.part ? 1 : dv.run;  // units: parts, or blocks
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int s = tid; s < a.c.S; s += AW * 32) {
+            const int n = kv_seq(a.c, a.starts, a.rows, s).n;
+            if (n < 0 || n > a.max_rows) atomicCAS(a.status, 0u, kDevKvStarts);
+        }
     const int w0 = (int)blockIdx.x * run, w1 = min(total, w0 + run);
     uint32_t phase = 0;  // bit i: parity of stage i
 
@@ -205,10 +246,20 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
         const int s = kv_find(sum, a.c.S, w);
         const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
         const int nb = max(1, (q.len + kKvBlock - 1) / kKvBlock);
-        const int h = (w - sum[s]) / nb, seg = sum[s] + h * nb;  // this (sequence, head)'s blocks: [seg, seg + nb)
-        const int b0 = w - seg, b1 = min(seg + nb, w1) - seg;
-        const bool first = b0 > 0, whole = b0 == 0 && b1 == nb;
-        w = seg + b1;
+        const int room = (sum[s + 1] - sum[s]) / a.c.H;  // units per head
+        const int h = (w - sum[s]) / room, seg = sum[s] + h * room;
+        int b0, b1;  // this (sequence, head)'s blocks [b0, b1) of nb
+        if (dv.part) {
+            const int each = (nb + room - 1) / room;
+            b0 = min(nb, (w - seg) * each);
+            b1 = min(nb, b0 + each);
+            w++;
+        } else {
+            b0 = w - seg;
+            b1 = min(nb, w1 - seg);
+            w = seg + b1;
+        }
+        const bool first = dv.part || b0 > 0, whole = b0 == 0 && b1 == nb;  // first: of the CTA's two places for parts
         const int pairs = q.n * G;
         if (tile * PT >= pairs) continue;
         const uint8_t* recs = a.c.codes + ((int64_t)s * a.c.H + h) * a.c.nb * (int64_t)REC;
@@ -318,9 +369,9 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 const uint4 vw = *reinterpret_cast<const uint4*>(rec + 32 * D + (np * 32 + lane) * 16);
                 const uint32_t ww[4] = {vw.x, vw.y, vw.z, vw.w};
 #pragma unroll
-                for (int f = 0; f < 2; f++)
+                for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
+                    for (int f = 0; f < 2; f++) {
                         const uint32_t v0 = kv_half2_lo(ww[2 * f + k]), v1 = kv_half2_hi(ww[2 * f + k]);
                         mma16816(o[2 * np + f], ah[k], v0, v1);
                         if (PT == 16) mma16816(o[2 * np + f], al[k], v0, v1);
@@ -409,19 +460,19 @@ __global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ Attn
     const KvAttnCall& a = P.a;
     // The kernel before lets this one start once its own wait for its predecessors is over, so what those wrote (the
     // lengths, the starts) may be read already; its own results may not.
-    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * a.c.H; });
+    const KvDivision dv = kv_divide(a, P.runs, sum, warp_sums);
     griddep_wait();
     griddep_launch_dependents();
     const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.G;
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-    const int nb = (sum[s + 1] - sum[s]) / a.c.H;
-    if (nb == 0 || gp >= q.n * G) return;
-    const int run = kv_run_length(sum[a.c.S], P.runs), seg = sum[s] + h * nb;
-    const int c0 = seg / run, c1 = (seg + nb - 1) / run;
+    const int room = (sum[s + 1] - sum[s]) / a.c.H;  // units per head
+    if (room == 0 || gp >= q.n * G) return;
+    const int seg = sum[s] + h * room, run = dv.part ? 1 : dv.run;
+    const int c0 = seg / run, c1 = (seg + room - 1) / run;
     if (c0 == c1) return;  // written by the CTA that had all of it
     const int tile = gp / PT, p = gp % PT;
     auto part = [&](int cta) {
-        return P.part + (((int64_t)tile * P.runs + cta) * 2 + (cta == c0 && seg >= cta * run ? 1 : 0)) * PT * (D + 2);
+        return P.part + (((int64_t)tile * P.runs + cta) * 2 + (!dv.part && cta == c0 ? 1 : 0)) * PT * (D + 2);
     };
     float M = -INFINITY;
 #pragma unroll 8

@@ -84,6 +84,21 @@ __device__ __forceinline__ void kv_prefix(int S, int* sum, int* warp_sums, F f)
         __syncthreads();
         return;
     }
+    if (S <= 32) {
+        if (warp == 0) {
+            const int x = lane < S ? f(lane) : 0;
+            int v = x;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, off);
+                if (lane >= off) v += u;
+            }
+            if (lane < S) sum[lane] = v - x;
+            if (lane == 31) sum[S] = v;
+        }
+        __syncthreads();
+        return;
+    }
     int carry = 0;
     for (int base = 0; base < S; base += blockDim.x) {
         const int s = base + tid;
