@@ -450,46 +450,75 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
     }
 }
 
-// Parts of a (sequence, head) that spans CTAs, in their order.  One CTA of
-// 128 threads per (pair, head, sequence).
-template <int D, int PT>
-__global__ void __launch_bounds__(128) k_kv_combine(const __grid_constant__ AttnParams P)
+// Parts of a (sequence, head) that spans CTAs: a pair's max and sum over the
+// parts by every warp that works on it, then the parts' outputs, four channels
+// per lane.  SHARE: one CTA per (pair, head, sequence), its warps taking the
+// parts in turn and added up in order -- few (sequence, head)s, many parts
+// each.  Else one CTA per (head, sequence) and a warp per pair.
+constexpr int CW_WARPS = 8;
+template <int D, int PT, bool SHARE>
+__global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_constant__ AttnParams P)
 {
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
+    __shared__ __align__(16) float total[SHARE ? CW_WARPS : 1][D];
     const KvAttnCall& a = P.a;
     // The kernel before lets this one start once its own wait for its predecessors is over, so what those wrote (the
     // lengths, the starts) may be read already; its own results may not.
     const KvDivision dv = kv_divide(a, P.runs, sum, warp_sums);
-    griddep_wait();
-    griddep_launch_dependents();
-    const int s = blockIdx.z, h = blockIdx.y, gp = blockIdx.x, d = threadIdx.x, G = a.G;
+    const int s = blockIdx.z, h = blockIdx.y, G = a.G;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
     const int room = (sum[s + 1] - sum[s]) / a.c.H;  // units per head
-    if (room == 0 || gp >= q.n * G) return;
     const int seg = sum[s] + h * room, run = dv.part ? 1 : dv.run;
-    const int c0 = seg / run, c1 = (seg + room - 1) / run;
-    if (c0 == c1) return;  // written by the CTA that had all of it
-    const int tile = gp / PT, p = gp % PT;
-    auto part = [&](int cta) {
-        return P.part + (((int64_t)tile * P.runs + cta) * 2 + (!dv.part && cta == c0 ? 1 : 0)) * PT * (D + 2);
-    };
-    float M = -INFINITY;
-#pragma unroll 8
-    for (int i = c0; i <= c1; i++) M = fmaxf(M, part(i)[p]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O = 0.f;
-#pragma unroll 8
-    for (int i = c0; i <= c1; i++) {
-        const float* src = part(i);
-        const float f = kv_ex2(src[p] - Ms);
-        L += src[PT + p] * f;
-        if (d < D) O += src[2 * PT + p * D + d] * f;
+    const int c0 = seg / run, n = room ? (seg + room - 1) / run - c0 + 1 : 0;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (n <= 1) return;  // nothing to answer, or written by the CTA that had all of it
+    for (int gp = SHARE ? (int)blockIdx.x : warp; gp < q.n * G; gp += SHARE ? (int)gridDim.x : CW_WARPS) {
+        const int tile = gp / PT, p = gp % PT;
+        auto part = [&](int i) {
+            return P.part + (((int64_t)tile * P.runs + c0 + i) * 2 + (!dv.part && i == 0 ? 1 : 0)) * PT * (D + 2);
+        };
+        float M = -INFINITY, L = 0.f;
+        for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[p]);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        const float Ms = M == -INFINITY ? 0.f : M;
+        for (int i = lane; i < n; i += 32) L += part(i)[PT + p] * kv_ex2(part(i)[p] - Ms);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        const bool none = M == -INFINITY && L == 0.f;
+        const float scale = none ? 0.f : __fdiv_rn(1.f, L);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int64_t row = q.row0 + gp / G;
+        const int head = h * G + gp % G;
+        float* dst = a.out + row * a.ldo + (int64_t)head * D;
+        if (lane < D / 4) {
+#pragma unroll 4
+            for (int i = SHARE ? warp : 0; i < n; i += SHARE ? CW_WARPS : 1) {
+                const float f = kv_ex2(part(i)[p] - Ms);
+                const float4 x = *reinterpret_cast<const float4*>(part(i) + 2 * PT + p * D + 4 * lane);
+                o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+            }
+        }
+        if (SHARE) {
+            if (lane < D / 4) *reinterpret_cast<float4*>(&total[warp][4 * lane]) = o;
+            __syncthreads();
+            for (int d = tid; d < D; d += CW_WARPS * 32) {
+                float x = 0.f;
+#pragma unroll
+                for (int i = 0; i < CW_WARPS; i++) x += total[SHARE ? i : 0][d];
+                dst[d] = x * scale;
+            }
+            __syncthreads();
+        } else if (lane < D / 4) {
+            const float x[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
+#pragma unroll
+            for (int i = 0; i < 4; i++) dst[4 * lane + i] = x[i];
+        }
+        if (P.lse && lane == 0 && (!SHARE || warp == 0)) P.lse[row * a.heads + head] = none ? INFINITY : M + log2f(L);
     }
-    const int64_t row = q.row0 + gp / G;
-    const int head = h * G + gp % G;
-    if (d < D) a.out[row * a.ldo + (int64_t)head * D + d] = M == -INFINITY && L == 0.f ? 0.f : O / L;
-    if (P.lse && d == 0) P.lse[row * a.heads + head] = M == -INFINITY && L == 0.f ? INFINITY : M + log2f(L);
 }
 
 // weights_out = weights + the p of every pair that sees the token.  One warp
@@ -575,8 +604,10 @@ cudaError_t launch_split(const AttnParams& P, const AttnPlan& p, cudaStream_t s)
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_attn<D, PT>, dim3((unsigned)p.runs, (unsigned)p.tiles), dim3(AW * 32), smem, s, P);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_kv_combine<D, PT>, dim3((unsigned)(P.a.max_rows * P.a.G), (unsigned)P.a.c.H, (unsigned)P.a.c.S),
-                      dim3(128), 0, s, P);
+    const int64_t pairs = P.a.max_rows * P.a.G, n = (int64_t)P.a.c.H * P.a.c.S;
+    const bool share = n * pairs <= 2 * p.runs;
+    return launch_pdl(share ? k_kv_combine<D, PT, true> : k_kv_combine<D, PT, false>,
+                      dim3((unsigned)(share ? pairs : 1), (unsigned)P.a.c.H, (unsigned)P.a.c.S), dim3(CW_WARPS * 32), 0, s, P);
 }
 
 }  // namespace
