@@ -206,15 +206,22 @@ __device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_
 }
 
 constexpr int kAttnStages = 2;  // blocks in flight per warp
-template <int D>
-constexpr size_t attn_smem_bytes() { return (size_t)AW * kAttnStages * kv_record_bytes(D); }
+// The tensor core cuts an accumulator's last bits at every step, always towards
+// zero; over the 80 steps that a warp takes for 8 x 65536 tokens that cost
+// 2e-6 of the output's norm, twice what fp32 arithmetic loses.  So a warp's
+// sums go to shared memory, rounded to nearest, every kFlush blocks.
+constexpr int kFlush = 8;
+// a warp's sums: m[PT], l[PT], O[PT][D + 8] (rows eight words apart modulo 32: float2 accesses without conflicts)
+template <int D, int PT>
+constexpr int attn_sum_floats() { return PT * (D + 10); }
+template <int D, int PT>
+constexpr size_t attn_smem_bytes() { return (size_t)AW * (kAttnStages * kv_record_bytes(D) + attn_sum_floats<D, PT>() * sizeof(float)); }
 
 template <int D, int PT>
 __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_constant__ AttnParams P)
 {
     constexpr int NST = kAttnStages, REC = kv_record_bytes(D), U = PT / 8, NT = D / 8;
-    constexpr int CW = NST * REC / 4;  // floats between two warps' rings
-    static_assert(PT * (D + 2) <= CW, "a warp's result fits its ring");
+    constexpr int CW = attn_sum_floats<D, PT>(), DS = D + 8;
     extern __shared__ __align__(128) uint8_t dyn[];
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
@@ -224,7 +231,9 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane / 4, c = lane % 4;
     const int tile = blockIdx.y, G = a.G;
     uint8_t* ring = dyn + warp * NST * REC;
-    float* comb = reinterpret_cast<float*>(dyn);  // at a segment's end, in each warp's ring: m[PT], l[PT], O[PT][D]
+    float* comb = reinterpret_cast<float*>(dyn + AW * NST * REC);
+    float* mine = comb + warp * CW;
+    float2* acc = reinterpret_cast<float2*>(mine + 2 * PT + r * DS + 2 * c);  // this lane's part of its pairs' sums
     if (tid == 0) abort_flag = 0;
     if (lane == 0) {
         for (int i = 0; i < NST; i++) mbar_init(&bars[warp][i], 1);
@@ -299,7 +308,36 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
 #pragma unroll
             for (int j = 0; j < 4; j++) o[i][j] = 0.f;
 
-        int st = 0;
+        float since[U];  // what the sums flushed so far have to be scaled by
+        bool flushed = false;
+#pragma unroll
+        for (int u = 0; u < U; u++) since[u] = 1.f;
+        auto flush = [&](float unit) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                float2 x[U];
+                x[0] = PT == 8 ? make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]) : make_float2(o[i][0], o[i][1]);
+                x[U - 1] = PT == 8 ? x[0] : make_float2(o[i][2], o[i][3]);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float2* at = acc + u * 4 * DS + 4 * i;  // (8 rows down: 8 DS floats)
+                    if (flushed) {
+                        const float2 y = *at;
+                        x[u].x = __fmaf_rn(y.x, since[u], x[u].x);
+                        x[u].y = __fmaf_rn(y.y, since[u], x[u].y);
+                    }
+                    x[u].x *= unit, x[u].y *= unit;
+                    *at = x[u];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[i][j] = 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) since[u] = 1.f;
+            flushed = true;
+        };
+
+        int st = 0, count = 0;
         float2 next = b0 + warp < b1 ? scales[b0 + warp] : make_float2(0.f, 0.f);
         for (int b = b0 + warp; b < b1; b += AW) {
             const float2 sc = next;
@@ -351,6 +389,8 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 const float ef = kv_pow2(max(-126, E - En));
                 E = En;
                 const float c0 = corr[0] * ef, c1 = PT == 8 ? c0 : corr[U - 1] * ef;
+                since[0] *= c0;
+                if (PT == 16) since[U - 1] *= c1;
 #pragma unroll
                 for (int i = 0; i < NT; i++) o[i][0] *= c0, o[i][1] *= c0, o[i][2] *= c1, o[i][3] *= c1;
             }
@@ -377,15 +417,13 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                         if (PT == 16) mma16816(o[2 * np + f], al[k], v0, v1);
                     }
             }
+            if (++count % kFlush == 0) flush(1.f);
             __syncwarp();
             issue(st);
             if (++st == NST) st = 0;
         }
-        // Join the warps, through the rings: every copy of the segment has been
-        // consumed, and each stage's phase bit is kept, so the next segment
-        // starts from stage 0 again.
-        float* mine = comb + warp * CW;
-        const float back = kv_pow2(E - 15);
+        // Join the warps.  (Every copy of the segment has been consumed, and each stage's phase bit is kept, so the next
+        // segment starts from stage 0 again.)
 #pragma unroll
         for (int u = 0; u < U; u++) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
@@ -395,19 +433,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 mine[PT + r + 8 * u] = l[u];
             }
         }
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-            float* row = mine + 2 * PT + r * D + 8 * i + 2 * c;
-            if (PT == 8) {
-                row[0] = (o[i][0] + o[i][2]) * back;
-                row[1] = (o[i][1] + o[i][3]) * back;
-            } else {
-                row[0] = o[i][0] * back;
-                row[1] = o[i][1] * back;
-                row[8 * D] = o[i][2] * back;
-                row[8 * D + 1] = o[i][3] * back;
-            }
-        }
+        flush(kv_pow2(E - 15));
         __syncthreads();
         // every thread the same: each warp's weight for each of its pairs, then four channels at a time
         float* part = P.part + (((int64_t)tile * P.runs + blockIdx.x) * 2 + (first ? 0 : 1)) * PT * (D + 2);
@@ -436,7 +462,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < AW; i++) {
-                    const float4 v = *reinterpret_cast<const float4*>(comb + i * CW + 2 * PT + pr * D + d);
+                    const float4 v = *reinterpret_cast<const float4*>(comb + i * CW + 2 * PT + pr * DS + d);
                     y.x += v.x * f[i], y.y += v.y * f[i], y.z += v.z * f[i], y.w += v.w * f[i];
                 }
                 y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
@@ -444,7 +470,6 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 else dst[d] = y.x, dst[d + 1] = y.y, dst[d + 2] = y.z, dst[d + 3] = y.w;
             }
         }
-        fence_proxy_async_smem();  // the next segment's copies follow these writes
         __syncthreads();
         if (abort_flag) return;
     }
@@ -598,7 +623,7 @@ AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
 template <int D, int PT>
 cudaError_t launch_split(const AttnParams& P, const AttnPlan& p, cudaStream_t s)
 {
-    constexpr size_t smem = attn_smem_bytes<D>();
+    constexpr size_t smem = attn_smem_bytes<D, PT>();
     static std::atomic<uint32_t> done{0};
     cudaError_t e = allow_smem(k_kv_attn<D, PT>, (int)smem, done);
     if (e != cudaSuccess) return e;
