@@ -546,45 +546,60 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
     }
 }
 
-// weights_out = weights + the p of every pair that sees the token.  One warp
-// per block of 32 tokens; a lane sums its 8 tokens over the pair tiles, then
-// the eight lanes that share them add up in a fixed order.
-template <int D>
+// weights_out = weights + the p of every pair that sees the token (at most PT
+// pairs).  A warp takes blocks of 32 tokens in turn; a lane adds up its rows'
+// p for its 8 tokens, then the eight lanes that share them add up by
+// butterfly.
+template <int D, int PT>
 __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ AttnParams P)
 {
+    constexpr int U = PT / 8;
     const KvAttnCall& a = P.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
-    const int s = blockIdx.z, h = blockIdx.y, b = blockIdx.x * AW + warp, G = a.G;
+    const int s = blockIdx.z, h = blockIdx.y, G = a.G;
+    // (the call's own earlier kernels wait for what came before it and write neither the lengths nor the queries)
+    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const int nb = (q.len + kKvBlock - 1) / kKvBlock, pairs = q.n > 0 && q.n <= a.max_rows ? q.n * G : 0;
+    const int64_t sh = (int64_t)s * a.c.H + h;
+    int b = blockIdx.x * AW + warp;
+    QFrag<D, PT> qf;
+    if (pairs && b < nb) qf.load(a, q, h, 0);
     griddep_wait();
     griddep_launch_dependents();
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-    if (kKvBlock * (int64_t)b >= q.len) return;
-    const int64_t sh = (int64_t)s * a.c.H + h;
-    const uint8_t* rec = a.c.codes + (sh * a.c.nb + b) * kv_record_bytes(D);
-    const float dk = a.c.scales[sh * a.c.nb + b].x;
-    const int pairs = q.n > 0 && q.n <= a.max_rows ? q.n * G : 0, t0 = kKvBlock * b + 8 * c;
-    float w[8];
+    if (b >= nb) return;
+    int lim[U];
+    float lse[U];
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = 0.f;
-    for (int tile = 0; tile * 8 < pairs; tile++) {
-        const int p = tile * 8 + r;
-        const int lim = p < pairs ? kv_limit(a, q, p / G) : 0;
-        if (!__any_sync(0xffffffffu, lim > kKvBlock * b)) continue;
-        QFrag<D, 8> qf;
-        qf.load(a, q, h, tile);
-        float z[1][8];
-        block_scores<D, 8>(qf, rec, z);
-        const float lse = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] += t0 + i < lim ? kv_ex2(z[0][i] * (qf.coef[0] * dk) - lse) : 0.f;
+    for (int u = 0; u < U; u++) {
+        const int p = r + 8 * u;
+        lim[u] = p < pairs ? kv_limit(a, q, p / G) : 0;
+        lse[u] = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
     }
+    for (; b < nb; b += gridDim.x * AW) {
+        const uint8_t* rec = a.c.codes + (sh * a.c.nb + b) * kv_record_bytes(D);
+        const float dk = a.c.scales[sh * a.c.nb + b].x;
+        const int t0 = kKvBlock * b + 8 * c;
+        float w[8], z[U][8];
+        if (pairs) block_scores<D, PT>(qf, rec, z);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 8; i++) {
+            w[i] = 0.f;
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], off);
-        if (r == i && t0 + i < q.len) {
-            const int64_t at = sh * a.c.cap + t0 + i;
-            a.weights_out[at] = (a.weights ? a.weights[at] : 0.f) + w[i];
+            for (int u = 0; u < U; u++) w[i] += t0 + i < lim[u] ? kv_ex2(z[u][i] * (qf.coef[u] * dk) - lse[u]) : 0.f;
+        }
+        // each step adds two rows and halves the tokens that a lane holds: lane (r, c) ends up with token 8 c + r
+#pragma unroll
+        for (int half = 4; half; half >>= 1)
+#pragma unroll
+            for (int i = 0; i < half; i++) {
+                const bool up = r & half;
+                const float give = up ? w[i] : w[i + half], keep = up ? w[i + half] : w[i];
+                w[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * half);
+            }
+        const int t = t0 + r;
+        if (t < q.len) {
+            const int64_t at = sh * a.c.cap + t;
+            a.weights_out[at] = (a.weights ? a.weights[at] : 0.f) + w[0];
         }
     }
 }
@@ -659,8 +674,11 @@ cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms,
         constexpr int D = decltype(d)::value;
         cudaError_t e = p.pt == 8 ? launch_split<D, 8>(P, p, s) : launch_split<D, 16>(P, p, s);
         if (e != cudaSuccess || !a.weights_out) return e;
-        return launch_pdl(k_kv_weights<D>, dim3((unsigned)((a.c.nb + AW - 1) / AW), (unsigned)a.c.H, (unsigned)a.c.S), dim3(AW * 32), 0,
-                          s, P);
+        // about four CTAs per SM, so that a warp's queries serve several blocks
+        const int64_t n = (int64_t)a.c.H * a.c.S, most = ((int64_t)a.c.nb + AW - 1) / AW;
+        const int64_t x = std::max<int64_t>(1, std::min(most, (4 * (int64_t)num_sms + n - 1) / n));
+        return launch_pdl(p.pt == 8 ? k_kv_weights<D, 8> : k_kv_weights<D, 16>, dim3((unsigned)x, (unsigned)a.c.H, (unsigned)a.c.S),
+                          dim3(AW * 32), 0, s, P);
     });
 }
 
