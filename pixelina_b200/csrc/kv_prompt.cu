@@ -653,43 +653,52 @@ __global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptP
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
     const KvAttnCall& a = P.a;
-    griddep_wait();
-    griddep_launch_dependents();
+    // (what came before the kernel that wrote the parts is over: that one waited for it before it let this one start)
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles(a, s); });
     const int gt = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, G = a.G;
-    if (gt >= sum[a.c.S]) return;
-    const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-    const int pr = blockIdx.z * 8 + (threadIdx.x >> 5), p = tile * kTileRows + pr;
-    if (p >= q.n * G) return;
-    int t0, t1;
-    prompt_keys(a, q, tile, 0, P.splits, t0, t1);
-    const int per = max(1, t1 - t0);
-    prompt_keys(a, q, tile, 0, 1, t0, t1);
-    const int used = (t1 + per - 1) / per;  // splits that had keys
+    int used = 0, p = 0, pr = 0;
+    KvSeq q{};
+    if (gt < sum[a.c.S]) {
+        const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
+        q = kv_seq(a.c, a.starts, a.rows, s);
+        pr = blockIdx.z * 8 + (threadIdx.x >> 5);
+        p = tile * kTileRows + pr;
+        if (p < q.n * G) {
+            int t0, t1;
+            prompt_keys(a, q, tile, 0, P.splits, t0, t1);
+            const int per = max(1, t1 - t0);
+            prompt_keys(a, q, tile, 0, 1, t0, t1);
+            used = max(1, (t1 + per - 1) / per);  // splits that had keys (none: the first says so)
+        }
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!used) return;
     const int64_t step = (int64_t)P.tiles * a.c.H * kTileRows * (D + 2);
     const float* part = P.part + ((int64_t)gt * a.c.H + h) * kTileRows * (D + 2);
-    float m = -INFINITY;
-    for (int i = 0; i < used; i++) m = fmaxf(m, part[i * step + pr]);
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < used; i += 32) m = fmaxf(m, part[i * step + pr]);
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[(D + 31) / 32];
+    for (int i = lane; i < used; i += 32) l += part[i * step + kTileRows + pr] * kv_ex2(part[i * step + pr] - ms);
 #pragma unroll
-    for (int u = 0; u < (D + 31) / 32; u++) o[u] = 0.f;
-    for (int i = 0; i < used; i++) {
-        const float* src = part + i * step;
-        const float f = kv_ex2(src[pr] - ms);
-        l += src[kTileRows + pr] * f;
-#pragma unroll
-        for (int u = 0; u < (D + 31) / 32; u++)
-            if (32 * u + lane < D) o[u] += src[2 * kTileRows + (int64_t)pr * D + 32 * u + lane] * f;
-    }
+    for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     const bool none = m == -INFINITY && l == 0.f;
+    const float f = none ? 0.f : __fdiv_rn(1.f, l);
     const int64_t row = q.row0 + p / G;
     const int head = h * G + p % G;
-    const float f = __fdiv_rn(1.f, l);
-#pragma unroll
-    for (int u = 0; u < (D + 31) / 32; u++)
-        if (32 * u + lane < D) a.out[row * a.ldo + (int64_t)head * D + 32 * u + lane] = none ? 0.f : o[u] * f;
+    if (lane < D / 4) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int i = 0; i < used; i++) {
+            const float w = kv_ex2(part[i * step + pr] - ms);
+            const float4 x = *reinterpret_cast<const float4*>(part + i * step + 2 * kTileRows + (int64_t)pr * D + 4 * lane);
+            o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
+        }
+        float* dst = a.out + row * a.ldo + (int64_t)head * D + 4 * lane;
+        dst[0] = o.x * f, dst[1] = o.y * f, dst[2] = o.z * f, dst[3] = o.w * f;
+    }
     if (P.lse && lane == 0) P.lse[row * a.heads + head] = none ? INFINITY : m + log2f(l);
 }
 
