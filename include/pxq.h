@@ -405,8 +405,9 @@ PXQ_API int pxq_attention(const float* q, size_t q_rows, const float* k, const f
  * depends on the rows alone, not on how they were cut into appends.
  *
  * The lengths live on the device: a captured step advances them on every
- * replay.  Calls that write a cache (append, truncate, evict into it) must be
- * ordered against every other call on it; calls that read one may overlap.
+ * replay.  Calls that write a cache (create, append, truncate, evict into it)
+ * must be ordered against every other call on it; calls that read one may
+ * overlap.
  * Errors that only the device can see (bounds outside the arrays, an append
  * beyond the capacity) leave the cache as it was and are reported by
  * pxq_synchronize as PXQ_ERR_DEVICE_STATUS.
@@ -448,7 +449,8 @@ PXQ_API int pxq_kv_truncate(pxq_kv_cache* c, const int32_t* lengths, void* strea
 /* The values the cache stands for: tokens [first[s], first[s] + count) of
  * every sequence (first: device int32, NULL: 0) into k and v (device fp32
  * [sequences][count][kv_heads * head_dim]; either may be NULL).  Rows of
- * tokens past a sequence's length are not written. */
+ * tokens past a sequence's length, and of a sequence whose first is negative,
+ * are not written. */
 PXQ_API int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t count, float* k, float* v, void* stream);
 
 /* Attention of q's rows (device fp32, stride ldq) over the cache: pxq_attention
@@ -462,7 +464,7 @@ PXQ_API int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t coun
  * weight that each cached token received from the rows and the heads that
  * share its kv head, added to `weights` (same shape; NULL: zeros; may be
  * weights_out itself).  Entries past a sequence's length are not touched.
- * heads must be a multiple of the cache's kv_heads. */
+ * heads must be a multiple of the cache's kv_heads; output may not overlap q. */
 PXQ_API int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t rows, const int32_t* starts,
                              size_t max_rows, size_t heads, int causal, float* output, size_t ldo, const float* weights,
                              float* weights_out, void* stream);

@@ -1481,7 +1481,9 @@ int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t r
     if (int rc = check_kv_rows(c, rows, starts)) return rc;
     if (!starts) max_rows = rows / (size_t)c->v.S;
     if (!max_rows || max_rows > rows) return fail(PXQ_ERR_INVALID, "max_rows %zu outside [1, rows = %zu]", max_rows, rows);
-    if (max_rows * (heads / (size_t)c->v.H) > 0x7fffffffu) return fail(PXQ_ERR_UNSUPPORTED, "rows x heads per group exceed INT32_MAX");
+    const size_t G = heads / (size_t)c->v.H;
+    if (max_rows * G > ((size_t)1 << 30) || (rows * G / 128 + c->v.S) * c->v.H > 0x7fffffffu)
+        return fail(PXQ_ERR_UNSUPPORTED, "rows x heads are more than one launch holds");
     DeviceCtx* d;
     if (int rc = ensure_device(&d)) return rc;
     if (int rc = check_kv(c)) return rc;

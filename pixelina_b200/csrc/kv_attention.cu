@@ -39,7 +39,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 struct AttnParams {
     KvAttnCall a;
-    float* part;   // partial results: [pair tile][CTA][2] x {m[PT], l[PT], O[PT][D]}
+    float* part;   // partial results: [pair tile][CTA][2] x {m[PT], l[PT], (O / l)[PT][D]}
     float* lse;    // [rows][heads] log2 of the softmax's denominator with its max, when weights are wanted
     int runs;      // CTAs of the flattened list
 };
@@ -134,7 +134,7 @@ struct QFrag {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // |x| 2^e < 2^15; a row of zeros, or one that is not finite, stays as it is
-            const int e = m > 0.f && m <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(m))) : 0;
+            const int e = m > 0.f && m <= FLT_MAX ? max(-113, min(110, 15 - kv_exponent(m))) : 0;
             const float up = kv_pow2(e);
             coef[u] = kv_log2_inv_sqrt(D) * kv_pow2(-e);
 #pragma unroll
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
         bool flushed = false;
 #pragma unroll
         for (int u = 0; u < U; u++) since[u] = 1.f;
-        auto flush = [&](float unit) {
+        auto flush = [&](const float (&unit)[U], float back) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 float2 x[U];
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                         x[u].x = __fmaf_rn(y.x, since[u], x[u].x);
                         x[u].y = __fmaf_rn(y.y, since[u], x[u].y);
                     }
-                    x[u].x *= unit, x[u].y *= unit;
+                    x[u].x = x[u].x * unit[u] * back, x[u].y = x[u].y * unit[u] * back;
                     *at = x[u];
                 }
 #pragma unroll
@@ -417,7 +417,12 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                         if (PT == 16) mma16816(o[2 * np + f], al[k], v0, v1);
                     }
             }
-            if (++count % kFlush == 0) flush(1.f);
+            if (++count % kFlush == 0) {
+                float one[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) one[u] = 1.f;
+                flush(one, 1.f);
+            }
             __syncwarp();
             issue(st);
             if (++st == NST) st = 0;
@@ -433,7 +438,11 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 mine[PT + r + 8 * u] = l[u];
             }
         }
-        flush(kv_pow2(E - 15));
+        // divided by their own sums already: the values' units could not hold the sums of the largest ones
+        float unit[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) unit[u] = l[u] == 0.f ? 0.f : __fdiv_rn(1.f, l[u]);
+        flush(unit, kv_pow2(E - 15));
         __syncthreads();
         // every thread the same: each warp's weight for each of its pairs, then four channels at a time
         float* part = P.part + (((int64_t)tile * P.runs + blockIdx.x) * 2 + (first ? 0 : 1)) * PT * (D + 2);
@@ -445,15 +454,15 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
         const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
         for (int i = 0; i < AW; i++) {
-            f[i] = kv_ex2(f[i] - Ms);
-            L += comb[i * CW + PT + pr] * f[i];
+            f[i] = kv_ex2(f[i] - Ms) * comb[i * CW + PT + pr];
+            L += f[i];
         }
         if (gp < pairs) {
             const bool none = M == -INFINITY && L == 0.f;  // no token seen; the max is asked too, so that a NaN sum stays NaN
             const int64_t row = q.row0 + gp / G;
             const int head = h * G + gp % G;
             float* dst = whole ? a.out + row * a.ldo + (int64_t)head * D : part + 2 * PT + pr * D;
-            const float scale = none ? 0.f : whole ? __fdiv_rn(1.f, L) : 1.f;
+            const float scale = none ? 0.f : __fdiv_rn(1.f, L);
             if (tid % TPP == 0) {
                 if (!whole) part[pr] = M, part[PT + pr] = L;
                 else if (P.lse) P.lse[row * a.heads + head] = none ? INFINITY : M + log2f(L);
@@ -463,9 +472,9 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
 #pragma unroll
                 for (int i = 0; i < AW; i++) {
                     const float4 v = *reinterpret_cast<const float4*>(comb + i * CW + 2 * PT + pr * DS + d);
-                    y.x += v.x * f[i], y.y += v.y * f[i], y.z += v.z * f[i], y.w += v.w * f[i];
+                    const float g = f[i] * scale;  // (at most 1: no sum outgrows the values)
+                    y.x += v.x * g, y.y += v.y * g, y.z += v.z * g, y.w += v.w * g;
                 }
-                y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
                 if (!whole || a.ovec) *reinterpret_cast<float4*>(dst + d) = y;
                 else dst[d] = y.x, dst[d + 1] = y.y, dst[d + 2] = y.z, dst[d + 3] = y.w;
             }
@@ -522,7 +531,7 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
         if (lane < D / 4) {
 #pragma unroll 4
             for (int i = SHARE ? warp : 0; i < n; i += SHARE ? CW_WARPS : 1) {
-                const float f = kv_ex2(part(i)[p] - Ms);
+                const float f = kv_ex2(part(i)[p] - Ms) * part(i)[PT + p] * scale;
                 const float4 x = *reinterpret_cast<const float4*>(part(i) + 2 * PT + p * D + 4 * lane);
                 o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
             }
@@ -534,13 +543,11 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
                 float x = 0.f;
 #pragma unroll
                 for (int i = 0; i < CW_WARPS; i++) x += total[SHARE ? i : 0][d];
-                dst[d] = x * scale;
+                dst[d] = x;
             }
             __syncthreads();
         } else if (lane < D / 4) {
-            const float x[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
-#pragma unroll
-            for (int i = 0; i < 4; i++) dst[4 * lane + i] = x[i];
+            dst[4 * lane] = o.x, dst[4 * lane + 1] = o.y, dst[4 * lane + 2] = o.z, dst[4 * lane + 3] = o.w;
         }
         if (P.lse && lane == 0 && (!SHARE || warp == 0)) P.lse[row * a.heads + head] = none ? INFINITY : M + log2f(L);
     }

@@ -93,7 +93,7 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 
 struct PromptParams {
     KvAttnCall a;
-    float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], O[128][D]
+    float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], (O / l)[128][D]
     float* lse;
     int tiles, splits;
     // weights (W): pair tiles [tile0, tile0 + tiles) of the batch; sums over a tile's pairs go to wpart [tile][head][wkeys]
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             row_sum[X][row] = top;
             named_bar_sync(3, 256);
             top = fmaxf(top, row_sum[X ^ 1][row]);
-            const int e = top > 0.f && top <= FLT_MAX ? max(-110, min(110, 15 - kv_exponent(top))) : 0;
+            const int e = top > 0.f && top <= FLT_MAX ? max(-113, min(110, 15 - kv_exponent(top))) : 0;
             const float up = kv_pow2(e);
             coef = kv_log2_inv_sqrt(D) * kv_pow2(-e);
 #pragma unroll
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             } else if (P.lse && p < pairs) {
                 P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] = none ? INFINITY : mn + log2f(l);
             }
-            const float scale = none ? 0.f : P.splits > 1 ? 1.f : __fdiv_rn(1.f, l);
+            const float scale = none || l == 0.f ? 0.f : __fdiv_rn(1.f, l);
             const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
             // every product is done: the row goes through smem, out by one bulk copy (or, unaligned, plain stores)
             float* dst = P.splits > 1 ? part + 2 * kTileRows + (int64_t)row * D : a.out + (int64_t)(q.row0 + p / G) * a.ldo + (int64_t)(h * G + p % G) * D;
@@ -692,12 +692,12 @@ __global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptP
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (int i = 0; i < used; i++) {
-            const float w = kv_ex2(part[i * step + pr] - ms);
+            const float w = kv_ex2(part[i * step + pr] - ms) * part[i * step + kTileRows + pr] * f;  // (at most 1)
             const float4 x = *reinterpret_cast<const float4*>(part + i * step + 2 * kTileRows + (int64_t)pr * D + 4 * lane);
             o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
         }
         float* dst = a.out + row * a.ldo + (int64_t)head * D + 4 * lane;
-        dst[0] = o.x * f, dst[1] = o.y * f, dst[2] = o.z * f, dst[3] = o.w * f;
+        dst[0] = o.x, dst[1] = o.y, dst[2] = o.z, dst[3] = o.w;
     }
     if (P.lse && lane == 0) P.lse[row * a.heads + head] = none ? INFINITY : m + log2f(l);
 }

@@ -341,6 +341,26 @@ def test_attention_over_blocks_of_very_different_scale(pxq, rows):
         assert max_abs_rel(got[i], want[i]) <= ATT_TOL
 
 
+@pytest.mark.parametrize("rows", [1, 9, 300])
+def test_attention_with_the_largest_numbers(pxq, rows):
+    """V up to fp32's largest numbers (sums of p V before the division would not fit), q up to 2^127 with K down at 2^-117."""
+    rng = np.random.default_rng(14)
+    heads, H, D, t = 2, 1, 64, 700
+    k = (2.0 ** -117 * rng.uniform(-1, 1, (t, H, D))).astype(np.float32)
+    v = (3.4e38 * rng.uniform(-1, 1, (t, H, D))).astype(np.float32)
+    q = (2.0 ** 118 * rng.uniform(-1, 1, (rows, heads, D))).astype(np.float32)
+    q[0] = 2.0 ** 127 * 1.9 * np.sign(q[0])
+    cache = pxq.KVCache(1, t, H, D)
+    cache.append(dev(k.reshape(t, -1)), dev(v.reshape(t, -1)))
+    got = pxq.kv_attention(dev(q.reshape(rows, -1)), cache, heads, causal=False).cpu().numpy().reshape(rows, heads, D)
+    pxq.synchronize()
+    want, _ = ref.attention(q, ref.values(k), ref.values(v), heads, False)
+    for i in range(1, rows):
+        assert max_abs_rel(got[i], want[i]) <= ATT_TOL
+    # row 0's scores go up to 2^17, where one step of fp32 is 2^-6: what is left to ask is that no number overflowed
+    assert np.isfinite(got[0]).all() and float(np.abs(got[0]).max()) <= 3.5e38
+
+
 def test_attention_bad_bounds(pxq):
     """A sequence with more rows than announced, or bounds outside q, is left alone and reported; the others are right."""
     import torch
