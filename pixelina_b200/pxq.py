@@ -168,10 +168,16 @@ def weight_bytes(inner: int, rows: int, wtype: int) -> int:
 
 # ------------------------------------------------------------ device side ---
 
-def _torch():
-    import torch  # noqa: WPS433 (device memory and streams only)
+_torch_module = None
 
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch  # noqa: WPS433 (device memory and streams only)
+
+        _torch_module = torch
+    return _torch_module
 
 
 def _stream_ptr(stream=None):
@@ -314,26 +320,33 @@ def attention(q, k, v, heads: int, kv_heads: int, ranges=None, query_offset: int
     return out
 
 
-_HERE = contextlib.nullcontext()
-
-
 def _on(stream):
     """Tensors made within belong to the stream that the call runs on."""
-    return _HERE if stream is None else _torch().cuda.stream(stream)
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
 
 
-def _rows(x, width: int, what: str, device):
+def _kv_stream(stream, device):
+    """Address of the stream, or of the device's current one."""
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw is not None else _torch().cuda.current_stream(device).cuda_stream
+
+
+def _rows(x, width: int, what: str, device, stream=None):
     """An fp32 matrix of `width` columns on `device` whose rows may be strided,
-    and its row stride (of one row: its width, whatever torch says)."""
-    torch = _torch()
-    if x.dtype is not torch.float32 or x.dim() != 2 or x.shape[1] != width or x.device != device:
+    and its row stride (of one row: its width, whatever torch says).  A copy,
+    where one is needed, is made on the stream that the call runs on."""
+    shape = x.shape
+    if x.dtype is not _torch().float32 or len(shape) != 2 or shape[1] != width or x.device != device:
         raise ValueError(f"{what} must be fp32 [rows, {width}] on {device}")
     if x.is_contiguous():
         return x, width
     ld, step = x.stride()
     if step != 1 or ld < width:
-        return x.contiguous(), width
-    return x, ld if x.shape[0] > 1 else width
+        with _on(stream):
+            return x.contiguous(), width
+    return x, ld if shape[0] > 1 else width
 
 
 def _whole(x, shape, dtype, what: str, device):
@@ -360,7 +373,7 @@ class KVCache:
             self.memory = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
         self.device = self.memory.device
         h = C.c_void_p()
-        _check(lib.pxq_kv_cache_create(self.memory.data_ptr(), sequences, capacity, kv_heads, head_dim, C.byref(h), _stream_ptr(stream)))
+        _check(lib.pxq_kv_cache_create(self.memory.data_ptr(), sequences, capacity, kv_heads, head_dim, C.byref(h), _kv_stream(stream, self.device)))
         self.handle = h
 
     def release(self) -> None:
@@ -387,24 +400,23 @@ class KVCache:
         h = self._live()
         with _on(stream):
             out = _torch().empty(self.sequences, dtype=_torch().int32, device=self.device)
-        _check(load().pxq_kv_cache_lengths(h, out.data_ptr(), _stream_ptr(stream)))
+        _check(load().pxq_kv_cache_lengths(h, out.data_ptr(), _kv_stream(stream, self.device)))
         return out
 
     def append(self, k, v, starts=None, stream=None) -> None:
         """Append rows k, v [rows, kv_heads*d]; rows [starts[s], starts[s+1]) go to sequence s."""
         h = self._live()
         width = self.kv_heads * self.head_dim
-        with _on(stream):
-            k, ldk = _rows(k, width, "k", self.device)
-            v, ldv = _rows(v, width, "v", self.device)
+        k, ldk = _rows(k, width, "k", self.device, stream)
+        v, ldv = _rows(v, width, "v", self.device, stream)
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
         _check(load().pxq_kv_append(h, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0], self._per_sequence(starts, "starts", 1),
-                                    _stream_ptr(stream)))
+                                    _kv_stream(stream, self.device)))
 
     def truncate(self, lengths=None, stream=None) -> None:
         """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them)."""
-        _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), _stream_ptr(stream)))
+        _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), _kv_stream(stream, self.device)))
 
     def read(self, first=None, count: Optional[int] = None, k=None, v=None, stream=None):
         """The values of tokens [first[s], first[s] + count) of every sequence:
@@ -419,7 +431,7 @@ class KVCache:
                 k = torch.zeros(shape, device=self.device) if k is None else k
                 v = torch.zeros(shape, device=self.device) if v is None else v
         _check(load().pxq_kv_read(h, self._per_sequence(first, "first"), count, _whole(k, shape, torch.float32, "k", self.device),
-                                  _whole(v, shape, torch.float32, "v", self.device), _stream_ptr(stream)))
+                                  _whole(v, shape, torch.float32, "v", self.device), _kv_stream(stream, self.device)))
         return k, v
 
 
@@ -432,23 +444,26 @@ def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[
     torch = _torch()
     h, device = cache._live(), cache.device
     width = heads * cache.head_dim
-    with _on(stream):
-        q, ldq = _rows(q, width, "q", device)
-        rows, ldo = q.shape[0], width
-        if out is None:
-            out = torch.empty((rows, width), dtype=torch.float32, device=device)
-        elif out.shape != (rows, width) or out.dtype is not torch.float32 or out.device != device or out.stride(1) != 1 or \
-                (rows > 1 and out.stride(0) < width):
-            raise ValueError(f"out must be fp32 [{rows}, {width}] on {device}, its rows contiguous")
-        elif rows > 1:
-            ldo = out.stride(0)
+    q, ldq = _rows(q, width, "q", device, stream)
+    rows, ldo = q.shape[0], width
+    if out is None:
+        if stream is None:
+            out = q.new_empty((rows, width))
+        else:
+            with _on(stream):
+                out = q.new_empty((rows, width))
+    elif out.shape != (rows, width) or out.dtype is not torch.float32 or out.device != device or out.stride(1) != 1 or \
+            (rows > 1 and out.stride(0) < width):
+        raise ValueError(f"out must be fp32 [{rows}, {width}] on {device}, its rows contiguous")
+    elif rows > 1:
+        ldo = out.stride(0)
     wi = wo = None
     if weights is not None or weights_out is not None:
         shape = (cache.sequences, cache.kv_heads, cache.capacity)
         wi = _whole(weights, shape, torch.float32, "weights", device)
         wo = _whole(weights_out, shape, torch.float32, "weights_out", device)
     _check(load().pxq_kv_attention(h, q.data_ptr(), ldq, rows, cache._per_sequence(starts, "starts", 1), max_rows or rows, heads,
-                                   1 if causal else 0, out.data_ptr(), ldo, wi, wo, _stream_ptr(stream)))
+                                   1 if causal else 0, out.data_ptr(), ldo, wi, wo, _kv_stream(stream, device)))
     return out
 
 
@@ -464,7 +479,7 @@ def kv_evict(src: KVCache, dst: KVCache, weights, keep: Optional[int] = None, re
     heads = (src.sequences, src.kv_heads)
     _check(load().pxq_kv_evict(a, b, _whole(weights, heads + (src.capacity,), torch.float32, "weights", src.device), keep, recent,
                                _whole(weights_out, (dst.sequences, dst.kv_heads, dst.capacity), torch.float32, "weights_out", src.device),
-                               _whole(kept, heads + (keep,), torch.int32, "kept", src.device), _stream_ptr(stream)))
+                               _whole(kept, heads + (keep,), torch.int32, "kept", src.device), _kv_stream(stream, src.device)))
 
 
 class _Uploaded:
