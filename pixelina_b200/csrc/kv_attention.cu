@@ -553,11 +553,11 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
     }
 }
 
-// weights_out = weights + the p of every pair that sees the token (at most PT
-// pairs).  A warp takes blocks of 32 tokens in turn; a lane adds up its rows'
-// p for its 8 tokens, then the eight lanes that share them add up by
+// weights_out = weights + the p of every pair that sees the token (at most T
+// tiles of PT pairs).  A warp takes blocks of 32 tokens in turn; a lane adds up
+// its rows' p for its 8 tokens, then the eight lanes that share them add up by
 // butterfly.
-template <int D, int PT>
+template <int D, int PT, int T>
 __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ AttnParams P)
 {
     constexpr int U = PT / 8;
@@ -569,30 +569,42 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
     const int nb = (q.len + kKvBlock - 1) / kKvBlock, pairs = q.n > 0 && q.n <= a.max_rows ? q.n * G : 0;
     const int64_t sh = (int64_t)s * a.c.H + h;
     int b = blockIdx.x * AW + warp;
-    QFrag<D, PT> qf;
-    if (pairs && b < nb) qf.load(a, q, h, 0);
+    QFrag<D, PT> qf[T];
+    if (pairs && b < nb) {
+#pragma unroll
+        for (int tile = 0; tile < T; tile++) qf[tile].load(a, q, h, tile);
+    }
     griddep_wait();
     griddep_launch_dependents();
     if (b >= nb) return;
-    int lim[U];
-    float lse[U];
+    int lim[T][U];
+    float lse[T][U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int p = r + 8 * u;
-        lim[u] = p < pairs ? kv_limit(a, q, p / G) : 0;
-        lse[u] = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
-    }
+    for (int tile = 0; tile < T; tile++)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = tile * PT + r + 8 * u;
+            lim[tile][u] = p < pairs ? kv_limit(a, q, p / G) : 0;
+            lse[tile][u] = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
+        }
     for (; b < nb; b += gridDim.x * AW) {
         const uint8_t* rec = a.c.codes + (sh * a.c.nb + b) * kv_record_bytes(D);
         const float dk = a.c.scales[sh * a.c.nb + b].x;
         const int t0 = kKvBlock * b + 8 * c;
-        float w[8], z[U][8];
-        if (pairs) block_scores<D, PT>(qf, rec, z);
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            w[i] = 0.f;
+        for (int i = 0; i < 8; i++) w[i] = 0.f;
+        if (pairs) {
 #pragma unroll
-            for (int u = 0; u < U; u++) w[i] += t0 + i < lim[u] ? kv_ex2(z[u][i] * (qf.coef[u] * dk) - lse[u]) : 0.f;
+            for (int tile = 0; tile < T; tile++) {
+                float z[U][8];
+                block_scores<D, PT>(qf[tile], rec, z);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        w[i] += t0 + i < lim[tile][u] ? kv_ex2(z[u][i] * (qf[tile].coef[u] * dk) - lse[tile][u]) : 0.f;
+            }
         }
         // each step adds two rows and halves the tokens that a lane holds: lane (r, c) ends up with token 8 c + r
 #pragma unroll
@@ -622,6 +634,8 @@ cudaError_t by_dim(int D, F f)
     }
 }
 
+constexpr int64_t kSideBySide = 2048;  // blocks
+
 struct AttnPlan {
     bool prompt;
     int pt, tiles, runs;
@@ -634,8 +648,12 @@ AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
     const int64_t pairs = a.max_rows * a.G;
     p.pt = pairs <= 8 ? 8 : 16;
     p.tiles = (int)((pairs + p.pt - 1) / p.pt);
-    p.runs = kCtasPerSm * num_sms;
-    p.prompt = pairs > 16;
+    // 17 to 32 pairs also run here, as two tiles side by side, over short caches: k_kv_prompt takes about 8 us more to begin
+    // and end, but 25 % less per block (28 heads over 4, 4 rows: 13.6 us against 22.2 us over 512 blocks, 35.1 us against
+    // 31.2 us over 4096).  The lengths being unknown here, the capacity stands for them.
+    const int64_t blocks = (int64_t)a.c.S * a.c.H * a.c.nb;
+    p.prompt = pairs > 16 && (pairs > 32 || blocks > kSideBySide);  // (two tiles is what k_kv_weights takes)
+    p.runs = std::max(1, kCtasPerSm * num_sms / p.tiles);
     if (p.prompt) p.part_bytes = (kv_prompt_part_bytes(a, num_sms) + 255) / 256 * 256;
     else p.part_bytes = ((size_t)p.tiles * p.runs * 2 * p.pt * (a.c.D + 2) * sizeof(float) + 255) / 256 * 256;
     p.lse_bytes = a.weights_out ? (size_t)a.rows * a.heads * sizeof(float) : 0;
@@ -684,7 +702,7 @@ cudaError_t launch_kv_attention(const KvAttnCall& a, void* scratch, int num_sms,
         // about four CTAs per SM, so that a warp's queries serve several blocks
         const int64_t n = (int64_t)a.c.H * a.c.S, most = ((int64_t)a.c.nb + AW - 1) / AW;
         const int64_t x = std::max<int64_t>(1, std::min(most, (4 * (int64_t)num_sms + n - 1) / n));
-        return launch_pdl(p.pt == 8 ? k_kv_weights<D, 8> : k_kv_weights<D, 16>, dim3((unsigned)x, (unsigned)a.c.H, (unsigned)a.c.S),
+        return launch_pdl(p.pt == 8 ? k_kv_weights<D, 8, 1> : p.tiles == 1 ? k_kv_weights<D, 16, 1> : k_kv_weights<D, 16, 2>, dim3((unsigned)x, (unsigned)a.c.H, (unsigned)a.c.S),
                           dim3(AW * 32), 0, s, P);
     });
 }

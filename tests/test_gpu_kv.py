@@ -227,6 +227,10 @@ CASES = [
     ([513], [257], 2, 1, 128, True),
     ([1300, 1290], [300, 5], 16, 16, 80, False),         # several key tiles and pair tiles
     ([260], [260], 3, 3, 128, True),
+    ([700, 33], [4, 3], 28, 4, 128, True),               # 17 to 32 pairs: two tiles of 16 side by side
+    ([50, 900, 0], [17, 25, 4], 2, 2, 80, False),
+    ([500], [32], 1, 1, 64, True),
+    ([300, 40000], [2, 3], 8, 1, 64, True),              # the same over a cache too long for that
 ]
 
 
