@@ -32,6 +32,17 @@
 // 5.6e-6 of its norm, five times what fp32 arithmetic loses.  So O_i starts at
 // zero for every tile, and the rows' sums over tiles are kept in registers,
 // rounded to nearest.
+//
+// What bounds it: with hi and lo, four half-precision products per element.  A
+// 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 237 us, in which
+// the tensor cores are issued 248 TFLOP (tiles on the diagonal whole): 1.04
+// PFLOP/s at the power cap (985 W, 1.81 GHz), where a plain bf16 product
+// sustains 1.38.  A tile takes 3400 cycles for 2048 of products: softmax, PV
+// and the next QK of a parity follow one another (4200 + 600 + 1700 cycles for
+// two tiles).  A CTA needs 16000 cycles more to begin and end.
+// The roles' loops are kept short: unrolled over a tile they did not fit the
+// instruction caches together, and warps waited for instructions (123 -> 93 us
+// for 148 x 128 rows over 4096 keys, with the sums' warpgroup).
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"
