@@ -23,11 +23,11 @@
 // What bounds k_kv_attn: reading the cache once, 2 len D bytes per (sequence,
 // head).  8 x 49000 tokens, 28 heads over 4 of 128: 71 us, 5.7 TB/s of 6.5.
 // Per block of 32 tokens a warp has 64 products (8 cycles each and SM
-// quarter) and about 450 instructions, half of them turning codes into fp16;
-// with two warps per quarter (the sums and queries fill the registers) that is
-// just above what the memory delivers.  With little to read it is bound by its
-// chain -- lengths, queries, copies, join -- of some 4 us, and k_kv_combine's
-// of 3 us: 8 x 3000 tokens 13.6 us, 1 x 1000 8.6 us.
+// quarter) and, counted in the source, some 450 instructions, more than half of
+// them turning codes into fp16; the registers leave room for two warps per
+// quarter.  With little to read the two kernels' chains of dependent steps
+// bound it (lengths, queries, copies, join): 8 x 3000 tokens 13.7 us, 1 x 1000
+// 8.5 us.
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"

@@ -15,9 +15,10 @@
 //
 // All are bound by memory when there is much to move and by their chain of
 // dependent loads when there is little: appending 65536 rows (4 heads of 128)
-// 85 us = 3.9 TB/s, one row to each of 8 sequences 4.4 us; reading 8 x 8191
-// tokens 62 us = 5.4 TB/s; evicting 8 x 32768 tokens to 8191 103 us, of which
-// the selection, one CTA per (head, sequence), takes 28.
+// 85 us = 3.9 TB/s (with the truncation before it), truncating and appending
+// one row to each of 8 sequences 6.1 us; reading 8 x 8191 tokens 62 us = 5.4
+// TB/s; evicting 8 x 32768 tokens to 8191 103 us: the selection, one CTA per
+// (head, sequence), about 29 and the packing 78, each timed alone.
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(SEL_THREADS)
 // NB destination blocks per CTA: their tokens' places and scales are looked up
 // at once.  All loads of a block are issued before the first is used, and four
 // CTAs share an SM: the kernel waits for memory (8 x 32768 tokens to 8191, 4
-// heads of 128: 107 us with the selection, 155 us at two CTAs per SM).
+// heads of 128: 107 us with the selection when this was measured, 155 us at two CTAs per SM).
 template <int D, int NB>
 __global__ void __launch_bounds__(2 * D, 4) k_kv_compact(const __grid_constant__ KvView c, const __grid_constant__ KvView dst,
                                                       const int32_t* kept, int keep)

@@ -37,12 +37,14 @@
 // 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 237 us, in which
 // the tensor cores are issued 248 TFLOP (tiles on the diagonal whole): 1.04
 // PFLOP/s at the power cap (985 W, 1.81 GHz), where a plain bf16 product
-// sustains 1.38.  A tile takes 3400 cycles for 2048 of products: softmax, PV
-// and the next QK of a parity follow one another (4200 + 600 + 1700 cycles for
-// two tiles).  A CTA needs 16000 cycles more to begin and end.
+// sustains 1.38.  148 x 128 rows take 39.6 us over 2048 keys and 138.3 over
+// 8192: 2.06 us per tile of 128 keys and some 7 us to begin and end.
+// By clock64 a tile takes about 3400 cycles for 2048 of products: softmax 2900,
+// PV 1900 to 3100 after it, QK 1600 to 1900.
 // The roles' loops are kept short: unrolled over a tile they did not fit the
 // instruction caches together, and warps waited for instructions (123 -> 93 us
-// for 148 x 128 rows over 4096 keys, with the sums' warpgroup).
+// for 148 x 128 rows over 4096 keys, together with the sums' warpgroup and the
+// bulk copies of the codes).
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"
