@@ -15,8 +15,8 @@
 //
 // All are bound by memory when there is much to move and by their chain of
 // dependent loads when there is little: appending 65536 rows (4 heads of 128)
-// 85 us = 3.9 TB/s (with the truncation before it), truncating and appending
-// one row to each of 8 sequences 6.1 us; reading 8 x 8191 tokens 62 us = 5.4
+// 91 us = 3.7 TB/s (with the truncation before it), truncating and appending
+// one row to each of 8 sequences 7.5 us; reading 8 x 8191 tokens 62 us = 5.4
 // TB/s; evicting 8 x 32768 tokens to 8191 103 us: the selection, one CTA per
 // (head, sequence), about 29 and the packing 78, each timed alone.
 #include <algorithm>

@@ -140,10 +140,15 @@ __device__ __forceinline__ int kv_find(const int* sum, int S, int u)
 // Count this CTA as one that has read the lengths (called by one thread after
 // a barrier behind those reads).  Returns whether it is the last of the grid:
 // the one that may write them, as soon as it likes.  Leaves the ticket at zero.
+// The reads of every CTA come before the last one's writes: each count is a
+// release, and the last CTA alone, after it, acquires (an acquire in every CTA
+// empties the L1 caches: 99 us instead of 91 for 65536 rows).
 __device__ __forceinline__ bool kv_last_reader(uint32_t* ticket, uint32_t ctas)
 {
-    const uint32_t t = atomicAdd(ticket, 1u);
+    uint32_t t;
+    asm volatile("atom.release.gpu.global.add.u32 %0, [%1], 1;" : "=r"(t) : "l"(ticket) : "memory");
     if (t != ctas - 1) return false;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
     *ticket = 0;
     return true;
 }
