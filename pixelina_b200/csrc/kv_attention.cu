@@ -56,9 +56,10 @@ struct AttnParams {
 
 // Blocks of sequence s: 0 when it has no rows to answer.  An empty cache
 // counts one (fully masked) block, so that its rows get their zeros.
+template <bool EARLY>
 __device__ __forceinline__ int kv_attn_blocks(const KvAttnCall& a, int s)
 {
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const KvSeq q = kv_seq<EARLY>(a.c, a.starts, a.rows, s);
     if (q.n <= 0 || q.n > a.max_rows) return 0;
     return max(1, (q.len + kKvBlock - 1) / kKvBlock);
 }
@@ -75,6 +76,7 @@ struct KvDivision {
     int part;  // most blocks of a part, sum[s]: parts before sequence s; 0: the flattened list
     int run;   // flattened: blocks per CTA, sum[s]: blocks before sequence s
 };
+template <bool EARLY = false>
 __device__ __forceinline__ KvDivision kv_divide(const KvAttnCall& a, int runs, int* sum, int* warp_sums)
 {
     const int S = a.c.S, H = a.c.H, n = S * H;
@@ -86,17 +88,17 @@ __device__ __forceinline__ KvDivision kv_divide(const KvAttnCall& a, int runs, i
         return d;
     };
     if (S == 1) {
-        const int nb = kv_attn_blocks(a, 0);
+        const int nb = kv_attn_blocks<EARLY>(a, 0);
         const KvDivision d = decide(nb * H);
         if (threadIdx.x == 0) sum[0] = 0, sum[1] = (d.part ? (nb + d.part - 1) / d.part : nb) * H;
         __syncthreads();
         return d;
     }
-    kv_prefix(S, sum, warp_sums, [&](int s) { return kv_attn_blocks(a, s) * H; });
+    kv_prefix(S, sum, warp_sums, [&](int s) { return kv_attn_blocks<EARLY>(a, s) * H; });
     const KvDivision d = decide(sum[S]);
     if (d.part) {
         __syncthreads();  // everyone has read the total
-        kv_prefix(S, sum, warp_sums, [&](int s) { return (kv_attn_blocks(a, s) + d.part - 1) / d.part * H; });
+        kv_prefix(S, sum, warp_sums, [&](int s) { return (kv_attn_blocks<EARLY>(a, s) + d.part - 1) / d.part * H; });
     }
     return d;
 }
@@ -110,6 +112,8 @@ struct QFrag {
     uint32_t lo[PT == 16 ? D / 16 : 1][4];
     float coef[PT / 8];
 
+    // EARLY: the kernel has not waited for its predecessors yet (who wrote q is over, but L1 may hold older rows)
+    template <bool EARLY = false>
     __device__ __forceinline__ void load(const KvAttnCall& a, const KvSeq& q, int h, int tile)
     {
         const int lane = lane_id(), r = lane / 4, c = lane % 4, G = a.G, pairs = q.n * G;
@@ -125,7 +129,8 @@ struct QFrag {
                 for (int k = 0; k < D / 16; k++) {
                     const int d = k < D / 64 * 4 ? 64 * (k / 4) + 16 * c + 4 * (k % 4) : D / 64 * 64 + 4 * c;
                     float4 v;
-                    if (decltype(vec)::value) v = *reinterpret_cast<const float4*>(src + d);
+                    if (decltype(vec)::value) v = EARLY ? __ldcg(reinterpret_cast<const float4*>(src + d)) : *reinterpret_cast<const float4*>(src + d);
+                    else if (EARLY) v = make_float4(__ldcg(src + d), __ldcg(src + d + 1), __ldcg(src + d + 2), __ldcg(src + d + 3));
                     else v = make_float4(src[d], src[d + 1], src[d + 2], src[d + 3]);
                     x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
                 }
@@ -509,10 +514,10 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
     const KvAttnCall& a = P.a;
     // The kernel before lets this one start once its own wait for its predecessors is over, so what those wrote (the
     // lengths, the starts) may be read already; its own results may not.
-    const KvDivision dv = kv_divide(a, P.runs, sum, warp_sums);
+    const KvDivision dv = kv_divide<true>(a, P.runs, sum, warp_sums);
     const int s = blockIdx.z, h = blockIdx.y, G = a.G;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const KvSeq q = kv_seq<true>(a.c, a.starts, a.rows, s);
     const int room = (sum[s + 1] - sum[s]) / a.c.H;  // units per head
     const int seg = sum[s] + h * room, run = dv.part ? 1 : dv.run;
     const int c0 = seg / run, n = room ? (seg + room - 1) / run - c0 + 1 : 0;
@@ -575,14 +580,14 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
     const int s = blockIdx.z, h = blockIdx.y, G = a.G;
     // (the call's own earlier kernels wait for what came before it and write neither the lengths nor the queries)
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const KvSeq q = kv_seq<true>(a.c, a.starts, a.rows, s);
     const int nb = (q.len + kKvBlock - 1) / kKvBlock, pairs = q.n > 0 && q.n <= a.max_rows ? q.n * G : 0;
     const int64_t sh = (int64_t)s * a.c.H + h;
     int b = blockIdx.x * AW + warp;
     QFrag<D, PT> qf[T];
     if (pairs && b < nb) {
 #pragma unroll
-        for (int tile = 0; tile < T; tile++) qf[tile].load(a, q, h, tile);
+        for (int tile = 0; tile < T; tile++) qf[tile].template load<true>(a, q, h, tile);
     }
     griddep_wait();
     griddep_launch_dependents();

@@ -51,16 +51,19 @@ __device__ __forceinline__ int kv_v_offset(int t, int d)
 
 // Sequence s of a ragged batch: its cached tokens and its rows
 // [row0, row0 + n) of the packed arrays.  n = -1: its bounds are not within
-// the arrays.
+// the arrays.  EARLY: a kernel that has not waited for its predecessors yet
+// (whoever wrote the lengths and the starts is over, but L1 may hold older
+// ones) takes them from L2.
 struct KvSeq {
     int len, n, row0;
 };
+template <bool EARLY = false>
 __device__ __forceinline__ KvSeq kv_seq(const KvView& c, const int32_t* starts, int64_t rows, int s)
 {
     KvSeq q;
-    q.len = c.lens[s];
+    q.len = EARLY ? __ldcg(c.lens + s) : c.lens[s];
     if (starts) {
-        const int a = starts[s], b = starts[s + 1];
+        const int a = EARLY ? __ldcg(starts + s) : starts[s], b = EARLY ? __ldcg(starts + s + 1) : starts[s + 1];
         q.row0 = a;
         q.n = (a < 0 || b < a || b > rows) ? -1 : b - a;
     } else {

@@ -115,9 +115,10 @@ struct PromptParams {
     int64_t wkeys;
 };
 
+template <bool EARLY = false>
 __device__ __forceinline__ int prompt_tiles(const KvAttnCall& a, int s)
 {
-    const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
+    const KvSeq q = kv_seq<EARLY>(a.c, a.starts, a.rows, s);
     if (q.n <= 0 || q.n > a.max_rows) return 0;
     return (q.n * a.G + kTileRows - 1) / kTileRows;  // (the host checks that rows x G fits)
 }
@@ -667,13 +668,13 @@ __global__ void __launch_bounds__(256) k_kv_join(const __grid_constant__ PromptP
     __shared__ int warp_sums[32];
     const KvAttnCall& a = P.a;
     // (what came before the kernel that wrote the parts is over: that one waited for it before it let this one start)
-    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles(a, s); });
+    kv_prefix(a.c.S, sum, warp_sums, [&](int s) { return prompt_tiles<true>(a, s); });
     const int gt = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, G = a.G;
     int used = 0, p = 0, pr = 0;
     KvSeq q{};
     if (gt < sum[a.c.S]) {
         const int s = kv_find(sum, a.c.S, gt), tile = gt - sum[s];
-        q = kv_seq(a.c, a.starts, a.rows, s);
+        q = kv_seq<true>(a.c, a.starts, a.rows, s);
         pr = blockIdx.z * 8 + (threadIdx.x >> 5);
         p = tile * kTileRows + pr;
         if (p < q.n * G) {
