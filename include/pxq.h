@@ -422,8 +422,8 @@ typedef struct pxq_kv_cache pxq_kv_cache;
 /* Device bytes that a cache needs (0: sizes it does not handle). */
 PXQ_API uint64_t pxq_kv_cache_bytes(size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim);
 
-/* An empty cache in `memory` (device, pxq_kv_cache_bytes() bytes, 256-byte
- * aligned), which stays the caller's and outlives the cache.  head_dim 64, 80
+/* An empty cache in `memory` (of the calling thread's device, pxq_kv_cache_bytes()
+ * bytes, 256-byte aligned), which stays the caller's and outlives the cache.  head_dim 64, 80
  * or 128; at most 1024 sequences, 4096 key/value heads, 2^30 tokens. */
 PXQ_API int pxq_kv_cache_create(void* memory, size_t sequences, size_t capacity, size_t kv_heads, size_t head_dim,
                                 pxq_kv_cache** out, void* stream);

@@ -1402,6 +1402,13 @@ int pxq_kv_cache_create(void* memory, size_t sequences, size_t capacity, size_t 
     if (reinterpret_cast<uintptr_t>(memory) % 256) return fail(PXQ_ERR_INVALID, "the cache's memory is not 256-byte aligned");
     DeviceCtx* d;
     if (int rc = ensure_device(&d)) return rc;
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, memory) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(PXQ_ERR_INVALID, "the cache's memory is not a device's");
+    }
+    if (at.type != cudaMemoryTypeDevice || at.device != t_device)
+        return fail(PXQ_ERR_INVALID, "the cache's memory is not on device %d", t_device);
     pxq_kv_cache* c = new (std::nothrow) pxq_kv_cache;
     if (!c) return fail(PXQ_ERR_NO_MEMORY, "no host memory");
     c->device = t_device;
@@ -1478,6 +1485,7 @@ int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t r
     const size_t width = heads * (size_t)c->v.D;
     if (ldq < width || ldo < width) return fail(PXQ_ERR_INVALID, "row stride below heads * head_dim = %zu", width);
     if (weights && !weights_out) return fail(PXQ_ERR_INVALID, "weights without weights_out");
+    if (output == q) return fail(PXQ_ERR_INVALID, "the output is q");
     if (int rc = check_kv_rows(c, rows, starts)) return rc;
     if (!starts) max_rows = rows / (size_t)c->v.S;
     if (!max_rows || max_rows > rows) return fail(PXQ_ERR_INVALID, "max_rows %zu outside [1, rows = %zu]", max_rows, rows);

@@ -628,3 +628,33 @@ def test_refusals(pxq):
         c.lengths()
     torch.cuda.synchronize()
     pxq.synchronize()
+
+
+def test_memory_that_is_not_the_devices_is_refused(pxq):
+    """Plain and pinned host memory: refused before anything is written to it."""
+    import ctypes as C
+
+    import torch
+
+    lib = pxq.load()
+    n = lib.pxq_kv_cache_bytes(1, 32, 1, 64)
+    h = C.c_void_p()
+    for pinned in (False, True):
+        memory = torch.full((n + 256,), 7, dtype=torch.uint8, pin_memory=pinned)
+        at = -(-memory.data_ptr() // 256) * 256
+        assert lib.pxq_kv_cache_create(at, 1, 32, 1, 64, C.byref(h), None) == pxq.ERR_INVALID
+        assert not h.value and bool((memory == 7).all())
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_output_that_is_q_is_refused(pxq, rows):
+    import torch
+
+    c = pxq.KVCache(1, 64, 2, 64)
+    x = torch.zeros((rows, 2 * 64), device="cuda")
+    c.append(x, x)
+    with pytest.raises(pxq.PxqError) as err:
+        pxq.kv_attention(x, c, 2, out=x)
+    assert err.value.code == pxq.ERR_INVALID
+    pxq.synchronize()
