@@ -169,12 +169,12 @@ struct QFrag {
 };
 
 // Scores of a block's 32 tokens: z[u][8] of pair row r + 8 u, tokens 8 c ..
-// 8 c + 7, before the scales.  rec: the block's record.
-template <int D, int PT>
-__device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_t* rec, float (&z)[PT / 8][8])
+// 8 c + 7, before the scales.  words(i): the lane's 16 bytes i (of D / 16) of
+// the block's K codes.
+template <int D, int PT, typename F>
+__device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, F words, float (&z)[PT / 8][8])
 {
     constexpr int J = D / 64;
-    const int lane = lane_id();
     float s[4][4];
 #pragma unroll
     for (int nt = 0; nt < 4; nt++)
@@ -185,7 +185,7 @@ __device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_
     for (int j = 0; j < J; j++) {
         uint4 w[4];
 #pragma unroll
-        for (int nt = 0; nt < 4; nt++) w[nt] = *reinterpret_cast<const uint4*>(rec + ((nt * J + j) * 32 + lane) * 16);
+        for (int nt = 0; nt < 4; nt++) w[nt] = words(nt * J + j);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
 #pragma unroll
@@ -198,7 +198,7 @@ __device__ __forceinline__ void block_scores(const QFrag<D, PT>& q, const uint8_
         }
     }
     if (D % 64 != 0) {
-        const uint4 w = *reinterpret_cast<const uint4*>(rec + 32 * 64 * J + lane * 16);
+        const uint4 w = words(4 * J);
         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) {
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             phase ^= 1u << st;
             const uint8_t* rec = ring + st * REC;
             float z[U][8];
-            block_scores<D, PT>(qf, rec, z);
+            block_scores<D, PT>(qf, [&](int i) { return *reinterpret_cast<const uint4*>(rec + (i * 32 + lane) * 16); }, z);
             // online softmax; lane (r, c) holds tokens 32 b + 8 c .. + 7 of its pairs
             const int t0 = kKvBlock * b + 8 * c;
             uint32_t ph[U][4], pl[U][4];
@@ -573,9 +573,10 @@ __global__ void __launch_bounds__(CW_WARPS * 32) k_kv_combine(const __grid_const
 // its rows' p for its 8 tokens, then the eight lanes that share them add up by
 // butterfly.
 template <int D, int PT, int T>
-__global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ AttnParams P)
+__global__ void __launch_bounds__(AW * 32, PT == 8 ? 3 : 2) k_kv_weights(const __grid_constant__ AttnParams P)
 {
     constexpr int U = PT / 8;
+    constexpr bool AHEAD = T == 1;  // (two tiles' queries leave no registers for a second block)
     const KvAttnCall& a = P.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
     const int s = blockIdx.z, h = blockIdx.y, G = a.G;
@@ -592,6 +593,14 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
     griddep_wait();
     griddep_launch_dependents();
     if (b >= nb) return;
+    if (!pairs) {  // nothing received
+        for (; b < nb; b += gridDim.x * AW) {
+            const int t = kKvBlock * b + lane;
+            const int64_t at = sh * a.c.cap + t;
+            if (t < q.len) a.weights_out[at] = a.weights ? a.weights[at] : 0.f;
+        }
+        return;
+    }
     int lim[T][U];
     float lse[T][U];
 #pragma unroll
@@ -602,24 +611,39 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
             lim[tile][u] = p < pairs ? kv_limit(a, q, p / G) : 0;
             lse[tile][u] = p < pairs ? P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] : 0.f;
         }
+    // the next block's codes are fetched while this one's products run (8 x 30000 tokens, 28 heads over 4 of 128, the
+    // attention included: 82 us; fetched when they are needed: 99)
+    uint4 next[D / 16];
+    float dnext = 0.f;
+    auto fetch = [&](int block) {
+        const uint4* rec = reinterpret_cast<const uint4*>(a.c.codes + (sh * a.c.nb + block) * kv_record_bytes(D)) + lane;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) next[i] = rec[32 * i];
+        dnext = a.c.scales[sh * a.c.nb + block].x;
+    };
+    if (AHEAD) fetch(b);
     for (; b < nb; b += gridDim.x * AW) {
-        const uint8_t* rec = a.c.codes + (sh * a.c.nb + b) * kv_record_bytes(D);
-        const float dk = a.c.scales[sh * a.c.nb + b].x;
-        const int t0 = kKvBlock * b + 8 * c;
+        uint4 rec[D / 16];
+        if (!AHEAD) fetch(b);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) rec[i] = next[i];
+        const float dk = dnext;
+        if (AHEAD && b + (int)gridDim.x * AW < nb) fetch(b + gridDim.x * AW);
+        const int t0 = kKvBlock * b + 8 * c, t = t0 + r;
+        const int64_t at = sh * a.c.cap + t;
+        const float before = a.weights && t < q.len ? a.weights[at] : 0.f;
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) w[i] = 0.f;
-        if (pairs) {
 #pragma unroll
-            for (int tile = 0; tile < T; tile++) {
-                float z[U][8];
-                block_scores<D, PT>(qf[tile], rec, z);
+        for (int tile = 0; tile < T; tile++) {
+            float z[U][8];
+            block_scores<D, PT>(qf[tile], [&](int i) { return rec[i]; }, z);
 #pragma unroll
-                for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                    for (int u = 0; u < U; u++)
-                        w[i] += t0 + i < lim[tile][u] ? kv_ex2(z[u][i] * (qf[tile].coef[u] * dk) - lse[tile][u]) : 0.f;
-            }
+                for (int u = 0; u < U; u++)
+                    w[i] += t0 + i < lim[tile][u] ? kv_ex2(z[u][i] * (qf[tile].coef[u] * dk) - lse[tile][u]) : 0.f;
         }
         // each step adds two rows and halves the tokens that a lane holds: lane (r, c) ends up with token 8 c + r
 #pragma unroll
@@ -630,11 +654,7 @@ __global__ void __launch_bounds__(AW * 32) k_kv_weights(const __grid_constant__ 
                 const float give = up ? w[i] : w[i + half], keep = up ? w[i + half] : w[i];
                 w[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * half);
             }
-        const int t = t0 + r;
-        if (t < q.len) {
-            const int64_t at = sh * a.c.cap + t;
-            a.weights_out[at] = (a.weights ? a.weights[at] : 0.f) + w[0];
-        }
+        if (t < q.len) a.weights_out[at] = before + w[0];
     }
 }
 
