@@ -454,7 +454,9 @@ PXQ_API int pxq_kv_truncate(pxq_kv_cache* c, const int32_t* lengths, void* strea
 PXQ_API int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t count, float* k, float* v, void* stream);
 
 /* Attention of q's rows (device fp32, stride ldq) over the cache: pxq_attention
- * on the values the cache stands for, to fp32 accuracy.  Sequence s has n =
+ * on the values the cache stands for, to fp32 accuracy (each row's: what it
+ * may not see, or gives next to no weight, costs it nothing, as long as the
+ * scales of the blocks that it sees differ by less than 2^128).  Sequence s has n =
  * starts[s + 1] - starts[s] <= max_rows rows (max_rows is ignored without
  * starts); causal: they are its last n tokens, row i sees the first
  * len - n + i + 1 of them; otherwise every row sees all len.  A row that sees

@@ -8,10 +8,11 @@
 // A pair is (query row, head of the kv head's group): pairs p = i * G + g are
 // the rows of the matrix products, so every key is read once for the group.
 //
-// Accuracy: codes are exact in fp16.  q (scaled per pair by a power of two to
-// below 2^15) and p are each the sum of two fp16 numbers, hi + lo, which
-// leaves 2^-22 of the value; products and sums are fp32.  So the result is
-// that of an fp32 computation at two half-precision products per element.
+// Accuracy: codes are exact in fp16.  q and p dv, brought to below 2^15 by
+// powers of two (p dv per pair: kv_unit), are each the sum of two fp16 numbers,
+// hi + lo.  That leaves 2^-22 of the value, or 2^-40 of the pair's largest where
+// that is more; products and sums are fp32.  So the result is that of an fp32
+// computation at two half-precision products per element.
 //
 //   k_kv_attn     split keys, up to 16 pairs per tile: a CTA takes a part of
 //                 a (sequence, head)'s blocks (kv_divide), its warps the
@@ -315,9 +316,10 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             lim[u] = p < pairs ? kv_limit(a, q, p / G) : 0;
         }
         float m[U], l[U], o[NT][4];
-        int E = -100;  // o is in units of 2^(E - 15); smaller scales lose nothing that fp32 sums would keep
+        float zv[U];  // the largest z + ev so far (kv_unit)
+        int E[U];     // o is in units of 2^(E - 15)
 #pragma unroll
-        for (int u = 0; u < U; u++) m[u] = -INFINITY, l[u] = 0.f;
+        for (int u = 0; u < U; u++) m[u] = zv[u] = -INFINITY, E[u] = kNoUnit, l[u] = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
         bool flushed = false;
 #pragma unroll
         for (int u = 0; u < U; u++) since[u] = 1.f;
-        auto flush = [&](const float (&unit)[U], float back) {
+        auto flush = [&](const float (&unit)[U], const float (&back)[U]) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 float2 x[U];
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                         x[u].x = __fmaf_rn(y.x, since[u], x[u].x);
                         x[u].y = __fmaf_rn(y.y, since[u], x[u].y);
                     }
-                    x[u].x = x[u].x * unit[u] * back, x[u].y = x[u].y * unit[u] * back;
+                    x[u].x = x[u].x * unit[u] * back[u], x[u].y = x[u].y * unit[u] * back[u];
                     *at = x[u];
                 }
 #pragma unroll
@@ -368,11 +370,10 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             // online softmax; lane (r, c) holds tokens 32 b + 8 c .. + 7 of its pairs
             const int t0 = kKvBlock * b + 8 * c;
             uint32_t ph[U][4], pl[U][4];
-            const int ev = kv_exponent(sc.y);
-            const int En = ev < 129 ? max(E, ev) : E;  // a NaN scale has exponent 129
-            const float up = sc.y * kv_pow2(15 - En);
+            const float ev = kv_scale_log(sc.y);
             float corr[U];
-            bool moved = En != E;
+            int step[U];  // of the unit's exponent
+            bool moved = false;
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const float k = qf.coef[u] * sc.x;
@@ -387,8 +388,14 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.f : mn;
                 corr[u] = kv_ex2(m[u] - ms);
-                moved |= mn != m[u];
+                zv[u] = fmaxf(zv[u], mx + ev);
+                const int En = kv_unit(zv[u], ms, mx > -INFINITY ? ev : -INFINITY, E[u]);
+                step[u] = E[u] - En;
+                const float2 inv = kv_unit_inverse(En);
+                const float up = sc.y * inv.x * inv.y;
+                moved |= mn != m[u] || step[u] != 0;
                 m[u] = mn;
+                E[u] = En;
                 float add = 0.f, y[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -401,9 +408,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 for (int i = 0; i < 4; i++) kv_split(y[2 * i], y[2 * i + 1], ph[u][i], pl[u][i]);
             }
             if (__any_sync(0xffffffffu, moved)) {
-                const float ef = kv_pow2(max(-126, E - En));
-                E = En;
-                const float c0 = corr[0] * ef, c1 = PT == 8 ? c0 : corr[U - 1] * ef;
+                const float c0 = kv_times_pow2(corr[0], step[0]), c1 = PT == 8 ? c0 : kv_times_pow2(corr[U - 1], step[U - 1]);
                 since[0] *= c0;
                 if (PT == 16) since[U - 1] *= c1;
 #pragma unroll
@@ -436,7 +441,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 float one[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) one[u] = 1.f;
-                flush(one, 1.f);
+                flush(one, one);
             }
             __syncwarp();
             issue(st);
@@ -454,10 +459,10 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             }
         }
         // divided by their own sums already: the values' units could not hold the sums of the largest ones
-        float unit[U];
+        float unit[U], back[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) unit[u] = l[u] == 0.f ? 0.f : __fdiv_rn(1.f, l[u]);
-        flush(unit, kv_pow2(E - 15));
+        for (int u = 0; u < U; u++) unit[u] = l[u] == 0.f ? 0.f : __fdiv_rn(1.f, l[u]), back[u] = kv_unit_value(E[u]);
+        flush(unit, back);
         __syncthreads();
         // every thread the same: each warp's weight for each of its pairs, then four channels at a time
         float* part = P.part + (((int64_t)tile * P.runs + blockIdx.x) * 2 + (first ? 0 : 1)) * PT * (D + 2);

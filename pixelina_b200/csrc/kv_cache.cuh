@@ -170,6 +170,47 @@ __device__ __forceinline__ float kv_pow2(int e) { return __int_as_float((e + 127
 // |x| < 2^this; -126 for 0, 129 for what is not finite
 __device__ __forceinline__ int kv_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 126; }
 
+// The unit of a row's value sums.  p dv goes to the tensor core as two fp16
+// numbers, whose floor is absolute, so each row has a unit of its own, 2^(E - 15)
+// with 2^E at least the row's largest p dv so far among the blocks that it
+// sees (p relative to its running max): a block that a row may not see, or to
+// which it gives next to no weight, takes no bits from the others.
+// w: the largest z + ev of these blocks (z a block's largest score, dv < 2^ev);
+// ms: the running max, 0 if -inf; top: the largest ev among those of them that
+// come new; E: the unit so far, kNoUnit at first.  E is never below top - 111,
+// so that dv over the unit stays below 2^127 whatever the p: a row that sees blocks whose
+// scales differ by more than 2^128 loses bits of the lesser ones.  Scores of
+// 2^20 and more leave too few bits to add ev to: their unit goes by dv alone.
+constexpr int kNoUnit = -239;
+__device__ __forceinline__ int kv_unit(float w, float ms, float top, int E)
+{
+    if (fabsf(ms) >= 1048576.f) return max(E, __float2int_ru(top));
+    return max(kNoUnit, __float2int_ru(fmaxf(w - ms, top - 111.f)));
+}
+// ev as kv_unit takes it: -inf for a NaN scale
+__device__ __forceinline__ float kv_scale_log(float dv)
+{
+    const int ev = kv_exponent(dv);
+    return ev < 129 ? (float)ev : -INFINITY;
+}
+// 2^(15 - E) as two factors, neither of which leaves fp32's range
+__device__ __forceinline__ float2 kv_unit_inverse(int E)
+{
+    const int e = 15 - E, a = e >> 1;
+    return make_float2(kv_pow2(a), kv_pow2(e - a));
+}
+// x * 2^d for 0 <= x <= 1 and a result that fits; 0 for d < -126.
+__device__ __forceinline__ float kv_times_pow2(float x, int d)
+{
+    return d < -126 ? 0.f : d > 100 ? x * kv_pow2(100) * kv_pow2(min(d - 100, 127)) : x * kv_pow2(d);
+}
+// 2^(E - 15), what the sums are multiplied by in the end (E >= -126, or nothing is seen)
+__device__ __forceinline__ float kv_unit_value(int E)
+{
+    const int e = max(-149, E - 15);
+    return e >= -126 ? kv_pow2(e) : __int_as_float(1 << (e + 149));
+}
+
 __device__ __forceinline__ uint32_t kv_pack(float a, float b)
 {
     const __half2 h = __floats2half2_rn(a, b);

@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_raw_empty[2], bar_s[2], bar_m[2], bar_w[2], bar_p[2][2], bar_o_full[2],
         bar_o_empty, bar_rows, bar_q, bar_fin;
     __shared__ float row_max[2][kTileRows], row_sum[2][kTileRows], row_gain[4][kTileRows];  // by tile's parity; gain by tile % 4
-    __shared__ int unit_exp[2];
+    __shared__ float row_zv[2][kTileRows];  // largest z + ev so far and unit (kv_unit), by tile's parity
+    __shared__ int row_unit[2][kTileRows];
     __shared__ float col_sum[W ? 2 : 1][2][4][kTileKeys];  // by tile's parity, alternating
     __shared__ uint32_t tmem_slot, abort_flag;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
@@ -340,17 +341,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             }
         } else {
         float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
-        int E = -100;                  // P_i holds p (dv / 2^(E - 15))
+        int E = kNoUnit;               // P_i holds p dv / 2^(E - 15)
         for (int i = X; i < n; i += 2) {
             const int key0 = (t0 + i) * kTileKeys;
             const float2 sc = next;
             next = fetch(i + 2);
-            const int x = kv_exponent(sc.y);
-            const int ev = __reduce_max_sync(0xffffffffu, x < 129 ? x : -100);  // 129: NaN
+            const float evs = kv_scale_log(sc.y);
             if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) break;
             tc_fence_after();
             const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
-            float mt = -INFINITY;
+            float mt = -INFINITY, wt = -INFINITY, et = -INFINITY;  // the tile's largest z, z + ev, ev
             // TMEM loads run one chunk of 16 tokens ahead of their use
             auto maxima = [&](auto masked) {
                 uint32_t r[2][16];
@@ -374,36 +374,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                         }
                     }
                     const float k = coef * __shfl_sync(0xffffffffu, sc.x, j);
-                    if (!decltype(masked)::value || mx != -INFINITY) mt = fmaxf(mt, mx * k);
+                    const float ev = __shfl_sync(0xffffffffu, evs, j);
+                    if (!decltype(masked)::value || mx != -INFINITY) {
+                        mt = fmaxf(mt, mx * k);
+                        wt = fmaxf(wt, mx * k + ev);
+                        et = fmaxf(et, ev);
+                    }
                 }
                 tmem_ld_wait_dep(r[0]);
             };
             if (full) maxima(std::false_type{});
             else maxima(std::true_type{});
             // the max and the unit of the tiles before, from the other parity
-            float mp = -INFINITY;
-            int Ep = -100;
+            float mp = -INFINITY, wp = -INFINITY;
+            int Ep = kNoUnit;
             if (i > 0) {
                 if (!mbar_wait(&bar_m[X ^ 1], ((i - 1) >> 1) & 1, &abort_flag, status, kDevTimeoutScaleFull)) break;
                 mp = row_max[X ^ 1][row];
-                Ep = unit_exp[X ^ 1];
+                wp = row_zv[X ^ 1][row];
+                Ep = row_unit[X ^ 1][row];
             }
             const float mn = fmaxf(mp, mt), ms = mn == -INFINITY ? 0.f : mn;
-            E = max(Ep, ev);
+            wt = fmaxf(wt, wp);
+            E = kv_unit(wt, ms, et, Ep);
             row_max[X][row] = mn;
-            if (row == 0) unit_exp[X] = E;
+            row_zv[X][row] = wt;
+            row_unit[X][row] = E;
             mbar_arrive(&bar_m[X]);
-            row_gain[i & 3][row] = kv_ex2(mp - ms) * kv_pow2(max(-126, Ep - E));
+            row_gain[i & 3][row] = kv_times_pow2(kv_ex2(mp - ms), Ep - E);
+            const float2 inv = kv_unit_inverse(E);
             l *= kv_ex2(m - ms);
             m = mn;
-            const float unit = kv_pow2(15 - E);
             float add0 = 0.f, add1 = 0.f;
             auto weigh = [&](auto masked) {
                 uint32_t r[2][16];
                 tmem_ld16(ts, r[0]);
 #pragma unroll 1
                 for (int j = 0; j < 4; j++) {
-                    const float k = coef * __shfl_sync(0xffffffffu, sc.x, j), y = unit * __shfl_sync(0xffffffffu, sc.y, j);
+                    const float k = coef * __shfl_sync(0xffffffffu, sc.x, j), y = __shfl_sync(0xffffffffu, sc.y, j) * inv.x * inv.y;
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         uint32_t hi[8], lo[8];
@@ -441,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         }
         row_max[X][row] = m;  // (read by nobody but the sums' warps any more)
         row_sum[X][row] = l;
-        if (row == 0) unit_exp[X] = E;
+        row_unit[X][row] = E;
         named_bar_sync(1, 384);
         }
     } else if (warp < 12) {
@@ -488,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] = none ? INFINITY : mn + log2f(l);
             }
             const float scale = none || l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-            const float back = kv_pow2(max(unit_exp[0], unit_exp[1]) - 15);
+            const float back = kv_unit_value(row_unit[(n - 1) & 1][row]);
             // every product is done: the row goes through smem, out by one bulk copy (or, unaligned, plain stores)
             float* dst = P.splits > 1 ? part + 2 * kTileRows + (int64_t)row * D : a.out + (int64_t)(q.row0 + p / G) * a.ldo + (int64_t)(h * G + p % G) * D;
             if (P.splits > 1 || a.ovec) {
