@@ -584,12 +584,15 @@ int run_matvec(DeviceCtx* d, pxq_weight* w, size_t row_first, size_t row_count, 
 // Scratch kept per (device, stream) for the fused quantize + matvec, so that
 // a steady decode loop makes no allocation (and no allocator node separates
 // its kernels in a captured graph).  Work on one stream is ordered, so one
-// buffer per stream is race-free.  A buffer is only replaced when a call
-// needs more; the old one is kept for the life of the process because a
-// captured graph may still name it.
+// buffer per stream is race-free as long as a call's kernels follow each other
+// there: host threads that share a stream take turns (`busy`, held by
+// CallScratch from the buffer's hand-over to the call's last launch).  A
+// buffer is only replaced when a call needs more; the old one is kept for the
+// life of the process because a captured graph may still name it.
 struct StreamScratch {
     void* ptr = nullptr;
     size_t bytes = 0;
+    std::mutex busy;  // taken before g_mutex, never while holding it
 };
 std::map<std::pair<int, cudaStream_t>, StreamScratch> g_stream_scratch;  // guarded by g_mutex
 std::vector<void*> g_retired_scratch;                                     // guarded by g_mutex
@@ -606,14 +609,20 @@ void reset_scratch_counters(int device)
     noalloc_clear_counters(device);
 }
 
-// The stream's scratch (at least `need` bytes), or null when no device memory
-// is left.  Growing it during a stream capture is allowed: like PyTorch's
+// The stream's scratch (at least `need` bytes), held by `busy`, or null when no
+// device memory is left.  Growing it during a stream capture is allowed: like PyTorch's
 // allocator, the cudaMalloc runs with this thread's capture mode relaxed, so
 // the buffer outlives the graph and no allocator node enters it.
-void* stream_scratch(int device, cudaStream_t s, size_t need)
+void* stream_scratch(int device, cudaStream_t s, size_t need, std::unique_lock<std::mutex>& busy)
 {
+    StreamScratch* held;
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        held = &g_stream_scratch[{device, s}];  // (a map's elements stay where they are)
+    }
+    busy = std::unique_lock<std::mutex>(held->busy);
     std::lock_guard<std::mutex> lock(g_mutex);
-    StreamScratch& e = g_stream_scratch[{device, s}];
+    StreamScratch& e = *held;
     if (e.bytes >= need) return e.ptr;
     size_t bytes = need > 2 * e.bytes ? need : 2 * e.bytes;
     if (bytes < ((size_t)4 << 20)) bytes = (size_t)4 << 20;
@@ -638,6 +647,60 @@ void* stream_scratch(int device, cudaStream_t s, size_t need)
     e.bytes = bytes;
     return p;
 }
+
+// One call's scratch, from get to the end of the object, which has to outlive
+// the call's last launch: the stream's buffer, no other host thread's call on
+// the stream in between, or stream-ordered memory of the call's own.  The
+// per-thread stream's handle names another stream in every thread, so a buffer
+// kept under it would be shared by streams that nothing orders: calls on it
+// have memory of their own.
+class CallScratch {
+public:
+    CallScratch() = default;
+    CallScratch(const CallScratch&) = delete;
+    CallScratch& operator=(const CallScratch&) = delete;
+    ~CallScratch()
+    {
+        if (own_) cudaFreeAsync(own_, s_);
+    }
+    // `need` bytes that begin with the matvec's counters, which are zero and which every call leaves zero.
+    int get(size_t need, cudaStream_t s)
+    {
+        if (s != cudaStreamPerThread) ptr_ = static_cast<uint8_t*>(stream_scratch(t_device, s, need, busy_));
+        if (ptr_) return PXQ_OK;
+        if (int rc = alone(need, s)) return rc;
+        PXQ_CUDA(cudaMemsetAsync(ptr_, 0, std::min(need, (size_t)kMvCounterRegion), s));
+        return PXQ_OK;
+    }
+    // `need` bytes without counters (past their region where the memory is the stream's).
+    int get_plain(size_t need, cudaStream_t s)
+    {
+        if (s != cudaStreamPerThread) ptr_ = static_cast<uint8_t*>(stream_scratch(t_device, s, kMvCounterRegion + need, busy_));
+        if (!ptr_) return alone(need, s);
+        ptr_ += kMvCounterRegion;
+        return PXQ_OK;
+    }
+    // Memory of the call's own.
+    int alone(size_t need, cudaStream_t s)
+    {
+        void* p = nullptr;
+        if (cudaMallocAsync(&p, need, s) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(PXQ_ERR_NO_MEMORY, "scratch allocation of %zu bytes failed", need);
+        }
+        own_ = p;
+        s_ = s;
+        ptr_ = static_cast<uint8_t*>(p);
+        return PXQ_OK;
+    }
+    uint8_t* ptr() const { return ptr_; }
+
+private:
+    uint8_t* ptr_ = nullptr;
+    void* own_ = nullptr;
+    cudaStream_t s_ = nullptr;
+    std::unique_lock<std::mutex> busy_;
+};
 
 int run_gemm(DeviceCtx* d, pxq_weight* w, size_t row_first, size_t row_count, const pxq_activation* a, float* output,
              size_t ldy, const float* bias, float* dump, cudaStream_t s, float* const* dsts = nullptr, int ndst = 0,
@@ -726,17 +789,9 @@ int run_matmul(DeviceCtx* d, pxq_weight* w, size_t row_first, size_t row_count, 
     if (force == 1 || (force == 0 && columns <= 8)) {
         if (!input) return fail(PXQ_ERR_INVALID, "null input");
         const MatvecPlan plan = plan_matvec(w->type, (int64_t)row_count, w->inner, (int64_t)columns, d->sms, true);
-        void* scratch = stream_scratch(t_device, s, plan.total_bytes);
-        const bool own = scratch == nullptr;
-        if (own && cudaMallocAsync(&scratch, plan.total_bytes, s) != cudaSuccess) {
-            cudaGetLastError();
-            return fail(PXQ_ERR_NO_MEMORY, "matvec scratch allocation of %zu bytes failed", plan.total_bytes);
-        }
-        if (own && plan.fused && plan.counter_bytes)  // fresh memory: no quantize kernel clears the counters
-            PXQ_CUDA(cudaMemsetAsync(static_cast<uint8_t*>(scratch) + plan.off_counters, 0, plan.counter_bytes, s));
-        cudaError_t e = matvec_fused(w, row_first, row_count, input, output, ldy, bias, plan, static_cast<uint8_t*>(scratch),
-                                     d->status, s);
-        if (own) cudaFreeAsync(scratch, s);
+        CallScratch scratch;
+        if (int rc = scratch.get(plan.total_bytes, s)) return rc;
+        cudaError_t e = matvec_fused(w, row_first, row_count, input, output, ldy, bias, plan, scratch.ptr(), d->status, s);
         if (e != cudaSuccess) return fail(PXQ_ERR_CUDA, "matvec launch failed: %s", cudaGetErrorString(e));
         return PXQ_OK;
     }
@@ -1225,15 +1280,9 @@ int pxq_matmul_gated(pxq_weight* w, const float* input, size_t columns, float* o
     if (w->type == kTypeQ5_K || w->type == kTypeQ6_K || w->inner % 256 == 0) {
         // one matvec: each CTA streams gate tile j and up tile j and writes silu(g) * u
         const MatvecPlan plan = plan_matvec(w->type, w->rows, w->inner, (int64_t)columns, d->sms, true, true);
-        void* scratch = stream_scratch(t_device, s, plan.total_bytes);
-        const bool own = scratch == nullptr;
-        if (own && cudaMallocAsync(&scratch, plan.total_bytes, s) != cudaSuccess) {
-            cudaGetLastError();
-            return fail(PXQ_ERR_NO_MEMORY, "gated matvec scratch allocation of %zu bytes failed", plan.total_bytes);
-        }
-        cudaError_t e = matvec_fused(w, 0, (size_t)w->rows, input, output, ldy, nullptr, plan, static_cast<uint8_t*>(scratch),
-                                     d->status, s);
-        if (own) cudaFreeAsync(scratch, s);
+        CallScratch scratch;
+        if (int rc = scratch.get(plan.total_bytes, s)) return rc;
+        cudaError_t e = matvec_fused(w, 0, (size_t)w->rows, input, output, ldy, nullptr, plan, scratch.ptr(), d->status, s);
         if (e != cudaSuccess) return fail(PXQ_ERR_CUDA, "gated matvec launch failed: %s", cudaGetErrorString(e));
         return PXQ_OK;
     }
@@ -1242,19 +1291,11 @@ int pxq_matmul_gated(pxq_weight* w, const float* input, size_t columns, float* o
     const MatvecPlan plan = plan_matvec(w->type, w->rows, w->inner, (int64_t)columns, d->sms, true);
     const size_t off_s = (plan.total_bytes + 255) & ~(size_t)255;
     const size_t need = off_s + (size_t)columns * (size_t)w->rows * 4;
-    void* scratch = stream_scratch(t_device, s, need);
-    const bool own = scratch == nullptr;
-    if (own && cudaMallocAsync(&scratch, need, s) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(PXQ_ERR_NO_MEMORY, "gated matvec scratch allocation of %zu bytes failed", need);
-    }
-    if (own && plan.fused && plan.counter_bytes)  // fresh memory: no quantize kernel clears the counters
-        PXQ_CUDA(cudaMemsetAsync(static_cast<uint8_t*>(scratch) + plan.off_counters, 0, plan.counter_bytes, s));
-    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + off_s);
-    cudaError_t e = matvec_fused(w, 0, (size_t)w->rows, input, sums, (size_t)w->rows, nullptr, plan,
-                                 static_cast<uint8_t*>(scratch), d->status, s);
+    CallScratch scratch;
+    if (int rc = scratch.get(need, s)) return rc;
+    float* sums = reinterpret_cast<float*>(scratch.ptr() + off_s);
+    cudaError_t e = matvec_fused(w, 0, (size_t)w->rows, input, sums, (size_t)w->rows, nullptr, plan, scratch.ptr(), d->status, s);
     if (e == cudaSuccess) e = counted(launch_gate_rows(sums, (int64_t)columns, F, output, (int64_t)ldy, s));
-    if (own) cudaFreeAsync(scratch, s);
     if (e != cudaSuccess) return fail(PXQ_ERR_CUDA, "gated matvec launch failed: %s", cudaGetErrorString(e));
     return PXQ_OK;
 }
@@ -1297,13 +1338,10 @@ int pxq_attention(const float* q, size_t q_rows, const float* k, const float* v,
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const size_t need = attention_scratch_bytes((int64_t)q_rows, (int64_t)heads, (int64_t)kv_heads, (int64_t)head_dim, (int64_t)k_rows, d->sms);
-    float* scratch = nullptr;
-    if (need) {
-        // past the matvec's counter region, which every call must leave zero
-        uint8_t* base = static_cast<uint8_t*>(stream_scratch(t_device, s, kMvCounterRegion + need));
-        if (!base) return fail(PXQ_ERR_NO_MEMORY, "attention scratch of %zu bytes", need);
-        scratch = reinterpret_cast<float*>(base + kMvCounterRegion);
-    }
+    CallScratch hold;
+    if (need)
+        if (int rc = hold.get_plain(need, s)) return rc;
+    float* scratch = reinterpret_cast<float*>(hold.ptr());
     const cudaError_t e = launch_attention(q, (int64_t)q_rows, k, v, (int64_t)k_rows, (int)heads, (int)kv_heads, (int)head_dim,
                                            ends, keys, causal, n, (int64_t)query_offset, output, scratch, need, d->sms, s);
     if (counted(e, need ? 2 : 1) != cudaSuccess) return fail(PXQ_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
@@ -1341,38 +1379,16 @@ int check_kv(const pxq_kv_cache* c)
     return PXQ_OK;
 }
 
-// One call's scratch: small needs from the stream's buffer (work on one stream
-// is ordered), large ones and those of a captured call stream-ordered -- a
-// graph then has memory of its own, whatever else was captured on the stream.
-struct KvScratch {
-    void* ptr = nullptr;
-    cudaStream_t s = nullptr;
-    bool own = false;
-    int get(size_t need, cudaStream_t stream)
-    {
-        s = stream;
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        PXQ_CUDA(cudaStreamIsCapturing(stream, &st));
-        if (st == cudaStreamCaptureStatusNone && need <= ((size_t)8 << 20)) {
-            // past the matvec's counter region, which every call must leave zero
-            uint8_t* base = static_cast<uint8_t*>(stream_scratch(t_device, stream, kMvCounterRegion + need));
-            if (base) ptr = base + kMvCounterRegion;
-        }
-        if (!ptr) {
-            own = true;
-            if (cudaMallocAsync(&ptr, need, stream) != cudaSuccess) {
-                cudaGetLastError();
-                return fail(PXQ_ERR_NO_MEMORY, "scratch of %zu bytes", need);
-            }
-        }
-        return PXQ_OK;
-    }
-    void put()
-    {
-        if (own) cudaFreeAsync(ptr, s);
-        own = false;
-    }
-};
+// A call's scratch: small needs from the stream's buffer, large ones and those
+// of a captured call stream-ordered -- a graph then has memory of its own,
+// whatever else was captured on the stream.
+int kv_scratch(CallScratch& scratch, size_t need, cudaStream_t s)
+{
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    PXQ_CUDA(cudaStreamIsCapturing(s, &st));
+    if (st == cudaStreamCaptureStatusNone && need <= ((size_t)8 << 20)) return scratch.get_plain(need, s);
+    return scratch.alone(need, s);
+}
 
 // The packed rows of a batch: with no starts, every sequence has the same number.
 int check_kv_rows(const pxq_kv_cache* c, size_t rows, const int32_t* starts)
@@ -1513,11 +1529,10 @@ int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t r
     a.weights = weights;
     a.weights_out = weights_out;
     a.status = d->status;
-    KvScratch scratch;
-    if (int rc = scratch.get(kv_attention_scratch_bytes(a, d->sms), s)) return rc;
+    CallScratch scratch;
+    if (int rc = kv_scratch(scratch, kv_attention_scratch_bytes(a, d->sms), s)) return rc;
     int launches = 0;
-    const cudaError_t e = launch_kv_attention(a, scratch.ptr, d->sms, s, &launches);
-    scratch.put();
+    const cudaError_t e = launch_kv_attention(a, scratch.ptr(), d->sms, s, &launches);
     if (counted(e, (uint64_t)launches) != cudaSuccess) return fail(PXQ_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
     return PXQ_OK;
 }
@@ -1537,13 +1552,12 @@ int pxq_kv_evict(const pxq_kv_cache* src, pxq_kv_cache* dst, const float* weight
     if (int rc = check_kv(src)) return rc;
     if (int rc = check_kv(dst)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    KvScratch scratch;
+    CallScratch scratch;
     if (!kept) {
-        if (int rc = scratch.get((size_t)src->v.S * src->v.H * keep * sizeof(int32_t), s)) return rc;
-        kept = static_cast<int32_t*>(scratch.ptr);
+        if (int rc = kv_scratch(scratch, (size_t)src->v.S * src->v.H * keep * sizeof(int32_t), s)) return rc;
+        kept = reinterpret_cast<int32_t*>(scratch.ptr());
     }
     const cudaError_t e = launch_kv_evict(src->v, dst->v, weights, (int64_t)keep, (int64_t)recent, weights_out, kept, s);
-    scratch.put();
     if (counted(e, 2) != cudaSuccess) return fail(PXQ_ERR_CUDA, "eviction launch failed: %s", cudaGetErrorString(e));
     return PXQ_OK;
 }
@@ -1626,7 +1640,10 @@ int pxq_debug_matvec_stall(pxq_weight* w, const float* input, size_t columns, fl
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     MatvecPlan plan = plan_matvec(w->type, w->rows, w->inner, (int64_t)columns, d->sms, true);
     plan.debug_stall = true;
-    void* scratch = static_scratch ? noalloc_scratch(t_device) : stream_scratch(t_device, s, plan.total_bytes);
+    CallScratch hold;
+    if (!static_scratch)
+        if (int rc = hold.get(plan.total_bytes, s)) return rc;
+    void* scratch = static_scratch ? noalloc_scratch(t_device) : hold.ptr();
     if (!scratch) return fail(PXQ_ERR_NO_MEMORY, "no scratch");
     if (static_scratch && plan.total_bytes > (size_t)PXQ_NOALLOC_SCRATCH_BYTES)
         return fail(PXQ_ERR_UNSUPPORTED, "the call does not fit the static scratch");

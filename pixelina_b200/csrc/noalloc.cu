@@ -31,7 +31,8 @@
 // Sharing: every call on a device uses the same array and it keeps the last
 // call's contents.  Two calls whose work overlaps on the GPU (different
 // streams without ordering) race on the array; order them on one stream or
-// with events.
+// with events.  Host threads that share a stream take turns, so that one
+// call's kernels follow each other there.
 #include <cstdio>
 #include <mutex>
 
@@ -44,6 +45,7 @@ static __device__ __align__(256) unsigned char g_noalloc_scratch[PXQ_NOALLOC_SCR
 
 constexpr int kMaxDevices = 16;
 std::mutex g_setup_mutex;
+std::mutex g_launch_mutex[kMaxDevices];  // held over a call's launches
 void* g_scratch_ptr[kMaxDevices] = {};
 
 }  // namespace
@@ -136,8 +138,12 @@ extern "C" int pxq_matvec_noalloc(pxq_weight* w, size_t row_first, size_t row_co
     void* scratch = pxq::noalloc_scratch(dev);
     if (!scratch) return noalloc_fail(PXQ_ERR_CUDA, "cudaGetSymbolAddress of the static scratch failed");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = pxq::matvec_fused(w, row_first, row_count, input, output, ldy, bias, plan,
-                                            static_cast<uint8_t*>(scratch), pxq::device_status(dev), s);
+    cudaError_t e;
+    {
+        std::lock_guard<std::mutex> lock(g_launch_mutex[dev]);
+        e = pxq::matvec_fused(w, row_first, row_count, input, output, ldy, bias, plan, static_cast<uint8_t*>(scratch),
+                              pxq::device_status(dev), s);
+    }
     if (e != cudaSuccess) {
         char msg[200];
         snprintf(msg, sizeof(msg), "kernel launch failed: %s", cudaGetErrorString(e));
