@@ -190,12 +190,15 @@ PXQ_API int pxq_quant_matmul(const unsigned char* weights, uint32_t type, const 
 PXQ_API int pxq_matmul_host(pxq_weight* w, size_t row_first, size_t row_count, const float* input, size_t columns,
                             float* output, size_t ldy);
 
-/* Wait for `stream` and report any bounded-wait timeout a kernel recorded
- * since the last call (PXQ_ERR_DEVICE_STATUS), then clear it.  On that
- * error it also waits for the whole device and zeroes the split-K counters
- * of every matvec scratch on it (the per-stream buffers and the
- * no-allocation array), which an interrupted matvec may leave non-zero;
- * later calls then compute correctly again. */
+/* Wait for `stream` and report (PXQ_ERR_DEVICE_STATUS) what kernels on the
+ * device recorded since it was last reported, to whichever caller asks first:
+ * - a bounded-wait timeout.  On that error it also waits for the whole device
+ *   and zeroes the split-K counters of every matvec scratch on it (the
+ *   per-stream buffers and the no-allocation array), which an interrupted
+ *   matvec may leave non-zero; later calls then compute correctly again.
+ * - else, the key/value cache's errors that only the device sees (bounds
+ *   outside the arrays, an append beyond the capacity); nothing is reset and
+ *   nothing else waited for. */
 PXQ_API int pxq_synchronize(void* stream);
 
 /* Reorder all-gathered output shards into one row-major output: src holds

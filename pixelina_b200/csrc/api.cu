@@ -60,7 +60,10 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
 struct DeviceCtx {
     bool ready = false;
     int sms = 0;
-    uint32_t* status = nullptr;  // device word written by kernels on a bounded-wait timeout
+    // device words written by kernels: the code of a bounded-wait timeout, then counts of the key/value cache's errors
+    // (kStatusKv*), which only grow
+    uint32_t* status = nullptr;
+    uint32_t kv_reported[kStatusKvWords] = {};  // of those counts (guarded by g_mutex)
     EncodeTiledFn encode = nullptr;
     // weight cache residency (guarded by g_mutex): the device bytes of cached
     // weights (raw rows + GEMM operand copies) and their budget
@@ -597,16 +600,29 @@ struct StreamScratch {
 std::map<std::pair<int, cudaStream_t>, StreamScratch> g_stream_scratch;  // guarded by g_mutex
 std::vector<void*> g_retired_scratch;                                     // guarded by g_mutex
 
-// Zero the counter region of every matvec scratch on `device`: the
-// per-stream buffers (current and retired) and the no-allocation array.  The
-// caller has synchronized the device.
+// Wait for the device and zero the counter region of every matvec scratch on
+// it: the per-stream buffers (current and retired) and the no-allocation
+// array.  Their calls are held off from before the wait to behind the writes.
 void reset_scratch_counters(int device)
 {
-    std::lock_guard<std::mutex> lock(g_mutex);
-    for (auto& kv : g_stream_scratch)
-        if (kv.first.first == device && kv.second.ptr) cudaMemset(kv.second.ptr, 0, kMvCounterRegion);
-    for (void* p : g_retired_scratch) cudaMemset(p, 0, kMvCounterRegion);
+    std::vector<StreamScratch*> current;
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        for (auto& kv : g_stream_scratch)
+            if (kv.first.first == device) current.push_back(&kv.second);
+    }
+    std::vector<std::unique_lock<std::mutex>> held;
+    for (StreamScratch* e : current) held.emplace_back(e->busy);  // (in the map's order; other calls hold one at a time)
+    std::unique_lock<std::mutex> noalloc = noalloc_hold(device);
+    cudaDeviceSynchronize();
+    for (StreamScratch* e : current)
+        if (e->ptr) cudaMemset(e->ptr, 0, kMvCounterRegion);
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        for (void* p : g_retired_scratch) cudaMemset(p, 0, kMvCounterRegion);
+    }
     noalloc_clear_counters(device);
+    cudaDeviceSynchronize();
 }
 
 // The stream's scratch (at least `need` bytes), held by `busy`, or null when no
@@ -851,6 +867,21 @@ void record_error(const char* msg)
 }  // namespace pxq
 
 namespace {
+
+// Wait for `s` and report a kernel that gave up a bounded wait.  A matvec
+// interrupted that way may leave counts in the split-K counters of its scratch,
+// which later fused calls (no quantize kernel to clear them) rely on finding
+// zero: every counter region on this device is zeroed once it is idle.
+int wait_stream(DeviceCtx* d, cudaStream_t s)
+{
+    PXQ_CUDA(cudaStreamSynchronize(s));
+    uint32_t st = 0;
+    PXQ_CUDA(cudaMemcpy(&st, d->status, 4, cudaMemcpyDeviceToHost));
+    if (!st) return PXQ_OK;
+    reset_scratch_counters(t_device);
+    cudaMemset(d->status, 0, 4);
+    return fail(PXQ_ERR_DEVICE_STATUS, "a kernel gave up waiting (status %u); scratch counters reset", st);
+}
 
 // per-thread stream for the host-buffer entry point (the reference's session
 // is thread-local too, src/backend_vulkan.cpp:86)
@@ -1465,7 +1496,7 @@ int pxq_kv_append(pxq_kv_cache* c, const float* k, size_t ldk, const float* v, s
     DeviceCtx* d;
     if (int rc = ensure_device(&d)) return rc;
     if (int rc = check_kv(c)) return rc;
-    PXQ_CUDA(counted(launch_kv_append(c->v, k, (int64_t)ldk, v, (int64_t)ldv, (int64_t)rows, starts, d->status,
+    PXQ_CUDA(counted(launch_kv_append(c->v, k, (int64_t)ldk, v, (int64_t)ldv, (int64_t)rows, starts, d->status + kStatusKv,
                                       static_cast<cudaStream_t>(stream))));
     return PXQ_OK;
 }
@@ -1611,21 +1642,20 @@ int pxq_synchronize(void* stream)
 {
     DeviceCtx* d;
     if (int rc = ensure_device(&d)) return rc;
-    PXQ_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-    uint32_t st = 0;
-    PXQ_CUDA(cudaMemcpy(&st, d->status, 4, cudaMemcpyDeviceToHost));
-    if (st) {
-        // A kernel gave up a bounded wait.  A matvec interrupted that way may
-        // leave counts in the split-K counters of its scratch, which later
-        // fused calls (no quantize kernel to clear them) rely on finding zero:
-        // once the device is idle, zero every counter region on this device.
-        cudaDeviceSynchronize();
-        reset_scratch_counters(t_device);
-        cudaMemset(d->status, 0, 4);
-        if (st == kDevKvStarts) return fail(PXQ_ERR_DEVICE_STATUS, "key/value cache: row bounds outside the arrays or above max_rows");
-        if (st == kDevKvCapacity) return fail(PXQ_ERR_DEVICE_STATUS, "key/value cache: an append exceeded the capacity and was dropped");
-        return fail(PXQ_ERR_DEVICE_STATUS, "a kernel gave up waiting (status %u); scratch counters reset", st);
+    if (int rc = wait_stream(d, static_cast<cudaStream_t>(stream))) return rc;
+    uint32_t count[kStatusKvWords];
+    PXQ_CUDA(cudaMemcpy(count, d->status + kStatusKv, sizeof(count), cudaMemcpyDeviceToHost));
+    bool bounds, capacity;
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        bounds = (int32_t)(count[kStatusKvStarts] - d->kv_reported[kStatusKvStarts]) > 0;
+        capacity = (int32_t)(count[kStatusKvCapacity] - d->kv_reported[kStatusKvCapacity]) > 0;
+        if (bounds) d->kv_reported[kStatusKvStarts] = count[kStatusKvStarts];
+        if (capacity) d->kv_reported[kStatusKvCapacity] = count[kStatusKvCapacity];
     }
+    if (bounds || capacity)
+        return fail(PXQ_ERR_DEVICE_STATUS, "key/value cache: %s%s%s", bounds ? "row bounds outside the arrays or above max_rows" : "",
+                    bounds && capacity ? "; " : "", capacity ? "an append exceeded the capacity and was dropped" : "");
     return PXQ_OK;
 }
 
@@ -1739,7 +1769,7 @@ int pxq_matmul_host(pxq_weight* w, size_t row_first, size_t row_count, const flo
     }
     cudaFreeAsync(xin, s);
     cudaFreeAsync(yout, s);
-    const int sync_rc = pxq_synchronize(s);
+    const int sync_rc = wait_stream(d, s);
     for (cudaEvent_t ev : evs) cudaEventDestroy(ev);
     if (ready) cudaEventDestroy(ready);
     if (fin_up) cudaEventDestroy(fin_up);

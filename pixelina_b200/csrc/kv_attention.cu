@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
     if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int s = tid; s < a.c.S; s += AW * 32) {
             const int n = kv_seq(a.c, a.starts, a.rows, s).n;
-            if (n < 0 || n > a.max_rows) atomicCAS(a.status, 0u, kDevKvStarts);
+            if (n < 0 || n > a.max_rows) atomicAdd(a.status + kStatusKv + kStatusKvStarts, 1u);
         }
     const int w0 = (int)blockIdx.x * run, w1 = min(total, w0 + run);
     uint32_t phase = 0;  // bit i: parity of stage i

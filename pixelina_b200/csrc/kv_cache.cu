@@ -196,7 +196,7 @@ __device__ __forceinline__ int kv_touched(const KvView& c, int len, int n)
 template <int D>
 __global__ void __launch_bounds__(2 * D, 4)
     k_kv_append(const __grid_constant__ KvView c, const float* k, int64_t ldk, const float* v, int64_t ldv,
-                int64_t rows, const int32_t* starts, int veck, uint32_t* status)
+                int64_t rows, const int32_t* starts, int veck, uint32_t* errors)
 {
     __shared__ int sum[kKvMaxSequences + 1];
     __shared__ int warp_sums[32];
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(2 * D, 4)
     for (int s = tid; s < c.S; s += blockDim.x) {
         const KvSeq q = kv_seq(c, starts, rows, s);
         if (bad || q.n < 0) {
-            atomicCAS(status, 0u, kDevKvStarts);
+            atomicAdd(errors + kStatusKvStarts, 1u);
             continue;
         }
         const int n = kv_touched(c, q.len, q.n);
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(2 * D, 4)
             c.held[s] = last;
             c.lens[s] = q.len + q.n;
         } else if (q.n > 0) {
-            atomicCAS(status, 0u, kDevKvCapacity);
+            atomicAdd(errors + kStatusKvCapacity, 1u);
         }
     }
 }
@@ -597,7 +597,7 @@ size_t kv_layout(int64_t S, int64_t H, int64_t D, int64_t cap, uint8_t* base, Kv
 }
 
 cudaError_t launch_kv_append(const KvView& c, const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t rows,
-                             const int32_t* starts, uint32_t* status, cudaStream_t s)
+                             const int32_t* starts, uint32_t* errors, cudaStream_t s)
 {
     // a sequence's n rows touch at most n / 32 + 2 blocks, and at most n
     const int64_t units = std::min(rows, rows / kKvBlock + 2 * (int64_t)c.S);
@@ -605,7 +605,7 @@ cudaError_t launch_kv_append(const KvView& c, const float* k, int64_t ldk, const
     return by_dim(c.D, [&](auto d) {
         constexpr int D = decltype(d)::value;
         return launch_pdl(k_kv_append<D>, dim3((unsigned)units, (unsigned)c.H), dim3(2 * D), 0, s, c, k, ldk, v, ldv, rows, starts,
-                          veck, status);
+                          veck, errors);
     });
 }
 

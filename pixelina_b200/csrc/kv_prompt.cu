@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     griddep_launch_dependents();
     kv_prefix(a.c.S, sum, warp_sums, [&](int s) {
         const KvSeq q = kv_seq(a.c, a.starts, a.rows, s);
-        if (!W && blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicCAS(a.status, 0u, kDevKvStarts);
+        if (!W && blockIdx.x == 0 && blockIdx.y == 0 && (q.n < 0 || q.n > a.max_rows)) atomicAdd(a.status + kStatusKv + kStatusKvStarts, 1u);
         return prompt_tiles(a, s);
     });
     tc_fence_after();

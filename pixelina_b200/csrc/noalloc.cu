@@ -90,6 +90,12 @@ void* noalloc_scratch(int device)
     return g_scratch_ptr[device];
 }
 
+// No call launches on the array while this is held.
+std::unique_lock<std::mutex> noalloc_hold(int device)
+{
+    return device >= 0 && device < kMaxDevices ? std::unique_lock<std::mutex>(g_launch_mutex[device]) : std::unique_lock<std::mutex>();
+}
+
 // Zero the counter region (after a call that a bounded wait interrupted may
 // have left counts in it; the caller has synchronized the device).  No-op
 // when the array was never set up on `device`.

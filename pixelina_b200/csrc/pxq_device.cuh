@@ -35,7 +35,6 @@ enum : uint32_t {
     kDevTimeoutScaleFull = 5,
     kDevTimeoutScaleEmpty = 6,
     kDevBadTmem = 7,
-    // 8 and 9: kDevKvStarts, kDevKvCapacity (pxq_internal.h)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p)

@@ -5,6 +5,7 @@
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <mutex>
 #include <cuda_fp16.h>
 
 namespace pxq {
@@ -68,8 +69,10 @@ cudaError_t launch_decode(const uint8_t* data, uint32_t type, int64_t count, flo
 
 // ---- noalloc.cu ------------------------------------------------------------
 // The static scratch array's device address on `device` (set up on first
-// use, with that device current), or null; and clearing its counter region.
+// use, with that device current), or null; holding its calls off; and clearing
+// its counter region.
 void* noalloc_scratch(int device);
+std::unique_lock<std::mutex> noalloc_hold(int device);
 cudaError_t noalloc_clear_counters(int device);
 
 // ---- matvec.cu -------------------------------------------------------------
@@ -191,9 +194,12 @@ cudaError_t launch_attention(const float* q, int64_t q_rows, const float* k, con
 // The 8-bit key/value cache (layout: kv_cache.cuh) in the caller's memory.
 constexpr int kKvBlock = 32;          // tokens per block
 constexpr int kKvMaxSequences = 1024;
-// status codes beside those of pxq_device.cuh, which the host tells apart
-constexpr uint32_t kDevKvStarts = 8;    // row bounds outside the arrays, or more rows than announced
-constexpr uint32_t kDevKvCapacity = 9;  // an append beyond the capacity
+// the cache's errors, counted in the device's status words from kStatusKv on
+// (the word before them holds a timeout's code)
+constexpr int kStatusKv = 1;
+constexpr int kStatusKvStarts = 0;    // row bounds outside the arrays, or more rows than announced
+constexpr int kStatusKvCapacity = 1;  // an append beyond the capacity
+constexpr int kStatusKvWords = 2;
 struct KvView {
     int32_t* lens;     // [S] tokens held
     int32_t* slot;     // [S] live tail slot
@@ -207,7 +213,7 @@ struct KvView {
 // Bytes of a cache's memory; when `base` is given, fills in the view.
 size_t kv_layout(int64_t S, int64_t H, int64_t D, int64_t cap, uint8_t* base, KvView* v);
 cudaError_t launch_kv_append(const KvView& c, const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t rows,
-                             const int32_t* starts, uint32_t* status, cudaStream_t s);
+                             const int32_t* starts, uint32_t* errors, cudaStream_t s);
 cudaError_t launch_kv_truncate(const KvView& c, const int32_t* lengths, cudaStream_t s);
 cudaError_t launch_kv_read(const KvView& c, const int32_t* first, int64_t count, float* k, float* v, cudaStream_t s);
 // weights [S][H][src.cap]; kept: int32 [S][H][keep], the source index of every kept token; weights_out
