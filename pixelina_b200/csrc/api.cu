@@ -1415,6 +1415,7 @@ int check_kv(const pxq_kv_cache* c)
 // whatever else was captured on the stream.
 int kv_scratch(CallScratch& scratch, size_t need, cudaStream_t s)
 {
+    if (!need) return PXQ_OK;
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     PXQ_CUDA(cudaStreamIsCapturing(s, &st));
     if (st == cudaStreamCaptureStatusNone && need <= ((size_t)8 << 20)) return scratch.get_plain(need, s);
