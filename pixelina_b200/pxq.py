@@ -358,6 +358,9 @@ def _whole(x, shape, dtype, what: str, device):
     return x.data_ptr()
 
 
+_PER_THREAD_STREAM = 2  # cudaStreamPerThread
+
+
 class KVCache:
     """An 8-bit key/value cache (pxq_kv_cache) for `sequences` sequences of up
     to `capacity` tokens; its memory is a torch tensor of its own."""
@@ -373,17 +376,35 @@ class KVCache:
             self.memory = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
         self.device = self.memory.device
         h = C.c_void_p()
-        _check(lib.pxq_kv_cache_create(self.memory.data_ptr(), sequences, capacity, kv_heads, head_dim, C.byref(h), _kv_stream(stream, self.device)))
+        at = _kv_stream(stream, self.device)
+        self._streams = {at}  # that torch knows to work on the memory
+        _check(lib.pxq_kv_cache_create(self.memory.data_ptr(), sequences, capacity, kv_heads, head_dim, C.byref(h), at))
         self.handle = h
 
     def release(self) -> None:
-        """Forget the cache; its memory goes back to torch."""
+        """Forget the cache; its memory goes back to torch, which hands it out
+        again when every stream that worked on it is done."""
         if self.handle:
+            self._settle()
             _check(load().pxq_kv_cache_release(self.handle))
             self.handle, self.memory = C.c_void_p(), None
 
+    def _settle(self):
+        # the per-thread stream's handle is another stream in every thread: torch could only wait for this thread's
+        if _PER_THREAD_STREAM in self._streams:
+            _torch().cuda.synchronize(self.device)
+
+    def _on_stream(self, stream):
+        """Address of the stream that a call runs on, which torch is told of where the memory is another stream's."""
+        at = _kv_stream(stream, self.device)
+        if at not in self._streams:
+            self.memory.record_stream(stream if stream is not None else _torch().cuda.current_stream(self.device))
+            self._streams.add(at)
+        return at
+
     def __del__(self):
         if getattr(self, "handle", None) and _lib is not None:
+            self._settle()
             _lib.pxq_kv_cache_release(self.handle)
             self.handle = C.c_void_p()
 
@@ -400,7 +421,7 @@ class KVCache:
         h = self._live()
         with _on(stream):
             out = _torch().empty(self.sequences, dtype=_torch().int32, device=self.device)
-        _check(load().pxq_kv_cache_lengths(h, out.data_ptr(), _kv_stream(stream, self.device)))
+        _check(load().pxq_kv_cache_lengths(h, out.data_ptr(), self._on_stream(stream)))
         return out
 
     def append(self, k, v, starts=None, stream=None) -> None:
@@ -412,11 +433,11 @@ class KVCache:
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
         _check(load().pxq_kv_append(h, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0], self._per_sequence(starts, "starts", 1),
-                                    _kv_stream(stream, self.device)))
+                                    self._on_stream(stream)))
 
     def truncate(self, lengths=None, stream=None) -> None:
         """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them)."""
-        _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), _kv_stream(stream, self.device)))
+        _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), self._on_stream(stream)))
 
     def read(self, first=None, count: Optional[int] = None, k=None, v=None, stream=None):
         """The values of tokens [first[s], first[s] + count) of every sequence:
@@ -431,7 +452,7 @@ class KVCache:
                 k = torch.zeros(shape, device=self.device) if k is None else k
                 v = torch.zeros(shape, device=self.device) if v is None else v
         _check(load().pxq_kv_read(h, self._per_sequence(first, "first"), count, _whole(k, shape, torch.float32, "k", self.device),
-                                  _whole(v, shape, torch.float32, "v", self.device), _kv_stream(stream, self.device)))
+                                  _whole(v, shape, torch.float32, "v", self.device), self._on_stream(stream)))
         return k, v
 
 
@@ -463,7 +484,7 @@ def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[
         wi = _whole(weights, shape, torch.float32, "weights", device)
         wo = _whole(weights_out, shape, torch.float32, "weights_out", device)
     _check(load().pxq_kv_attention(h, q.data_ptr(), ldq, rows, cache._per_sequence(starts, "starts", 1), max_rows or rows, heads,
-                                   1 if causal else 0, out.data_ptr(), ldo, wi, wo, _kv_stream(stream, device)))
+                                   1 if causal else 0, out.data_ptr(), ldo, wi, wo, cache._on_stream(stream)))
     return out
 
 
@@ -477,9 +498,10 @@ def kv_evict(src: KVCache, dst: KVCache, weights, keep: Optional[int] = None, re
     if weights is None:
         raise ValueError("weights are needed")
     heads = (src.sequences, src.kv_heads)
+    dst._on_stream(stream)
     _check(load().pxq_kv_evict(a, b, _whole(weights, heads + (src.capacity,), torch.float32, "weights", src.device), keep, recent,
                                _whole(weights_out, (dst.sequences, dst.kv_heads, dst.capacity), torch.float32, "weights_out", src.device),
-                               _whole(kept, heads + (keep,), torch.int32, "kept", src.device), _kv_stream(stream, src.device)))
+                               _whole(kept, heads + (keep,), torch.int32, "kept", src.device), src._on_stream(stream)))
 
 
 class _Uploaded:
