@@ -483,7 +483,7 @@ def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[
         shape = (cache.sequences, cache.kv_heads, cache.capacity)
         wi = _whole(weights, shape, torch.float32, "weights", device)
         wo = _whole(weights_out, shape, torch.float32, "weights_out", device)
-    _check(load().pxq_kv_attention(h, q.data_ptr(), ldq, rows, cache._per_sequence(starts, "starts", 1), max_rows or rows, heads,
+    _check(load().pxq_kv_attention(h, q.data_ptr(), ldq, rows, cache._per_sequence(starts, "starts", 1), rows if max_rows is None else max_rows, heads,
                                    1 if causal else 0, out.data_ptr(), ldo, wi, wo, cache._on_stream(stream)))
     return out
 

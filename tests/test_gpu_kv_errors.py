@@ -99,3 +99,14 @@ def test_a_host_product_does_not_take_the_caches_error(pxq):
     assert "capacity" in str(err.value)
     pxq.synchronize()
     W.release()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_max_rows_of_zero_is_refused(pxq, rows):
+    import torch
+
+    c = pxq.KVCache(1, 64, 2, 64)
+    x = torch.zeros((rows, 2 * 64), device="cuda")
+    with pytest.raises(pxq.PxqError) as err:
+        pxq.kv_attention(x, c, 2, starts=i32([0, rows]), max_rows=0)
+    assert err.value.code == pxq.ERR_INVALID
