@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 zv[u] = fmaxf(zv[u], mx + ev);
                 const int En = kv_unit(zv[u], ms, mx > -INFINITY ? ev : -INFINITY, E[u]);
                 step[u] = E[u] - En;
-                const float2 inv = kv_unit_inverse(En);
+                const float2 inv = kv_pow2_pair(15 - En);
                 const float up = sc.y * inv.x * inv.y;
                 moved |= mn != m[u] || step[u] != 0;
                 m[u] = mn;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 for (int i = 0; i < 4; i++) kv_split(y[2 * i], y[2 * i + 1], ph[u][i], pl[u][i]);
             }
             if (__any_sync(0xffffffffu, moved)) {
-                const float c0 = kv_times_pow2(corr[0], step[0]), c1 = PT == 8 ? c0 : kv_times_pow2(corr[U - 1], step[U - 1]);
+                const float c0 = kv_unit_step(corr[0], step[0]), c1 = PT == 8 ? c0 : kv_unit_step(corr[U - 1], step[U - 1]);
                 since[0] *= c0;
                 if (PT == 16) since[U - 1] *= c1;
 #pragma unroll

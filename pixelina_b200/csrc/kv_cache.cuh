@@ -181,7 +181,7 @@ __device__ __forceinline__ int kv_exponent(float x) { return (int)(__float_as_ui
 // so that dv over the unit stays below 2^127 whatever the p: a row that sees blocks whose
 // scales differ by more than 2^128 loses bits of the lesser ones.  Scores of
 // 2^20 and more leave too few bits to add ev to: their unit goes by dv alone.
-constexpr int kNoUnit = -239;
+constexpr int kNoUnit = -237;  // (15 - E stays below 253)
 __device__ __forceinline__ int kv_unit(float w, float ms, float top, int E)
 {
     if (fabsf(ms) >= 1048576.f) return max(E, __float2int_ru(top));
@@ -193,16 +193,18 @@ __device__ __forceinline__ float kv_scale_log(float dv)
     const int ev = kv_exponent(dv);
     return ev < 129 ? (float)ev : -INFINITY;
 }
-// 2^(15 - E) as two factors, neither of which leaves fp32's range
-__device__ __forceinline__ float2 kv_unit_inverse(int E)
+// 2^e, |e| <= 252, as two factors, neither of which leaves fp32's range
+__device__ __forceinline__ float2 kv_pow2_pair(int e)
 {
-    const int e = 15 - E, a = e >> 1;
+    const int a = e >> 1;
     return make_float2(kv_pow2(a), kv_pow2(e - a));
 }
-// x * 2^d for 0 <= x <= 1 and a result that fits; 0 for d < -126.
-__device__ __forceinline__ float kv_times_pow2(float x, int d)
+// what the sums so far are multiplied by as the unit's exponent falls by d (or rises by -d) and the running max's p
+// becomes corr
+__device__ __forceinline__ float kv_unit_step(float corr, int d)
 {
-    return d < -126 ? 0.f : d > 100 ? x * kv_pow2(100) * kv_pow2(min(d - 100, 127)) : x * kv_pow2(d);
+    const float2 f = kv_pow2_pair(max(-252, min(252, d)));
+    return corr * f.x * f.y;
 }
 // 2^(E - 15), what the sums are multiplied by in the end (E >= -126, or nothing is seen)
 __device__ __forceinline__ float kv_unit_value(int E)

@@ -401,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             row_zv[X][row] = wt;
             row_unit[X][row] = E;
             mbar_arrive(&bar_m[X]);
-            row_gain[i & 3][row] = kv_times_pow2(kv_ex2(mp - ms), Ep - E);
-            const float2 inv = kv_unit_inverse(E);
+            row_gain[i & 3][row] = kv_unit_step(kv_ex2(mp - ms), Ep - E);
+            const float2 inv = kv_pow2_pair(15 - E);
             l *= kv_ex2(m - ms);
             m = mn;
             float add0 = 0.f, add1 = 0.f;
