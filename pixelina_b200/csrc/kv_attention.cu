@@ -22,13 +22,13 @@
 //   k_kv_weights  the weights, from each pair's max and sum
 //
 // What bounds k_kv_attn: reading the cache once, 2 len D bytes per (sequence,
-// head).  8 x 49000 tokens, 28 heads over 4 of 128: 71 us, 5.7 TB/s of 6.5.
+// head).  8 x 49000 tokens, 28 heads over 4 of 128: 71.6 us, 5.6 TB/s of 6.5.
 // Per block of 32 tokens a warp has 64 products (8 cycles each and SM
-// quarter) and, counted in the source, some 450 instructions, more than half of
+// quarter) and, counted in the source, some 470 instructions, about half of
 // them turning codes into fp16; the registers leave room for two warps per
 // quarter.  With little to read the two kernels' chains of dependent steps
-// bound it (lengths, queries, copies, join): 8 x 3000 tokens 13.7 us, 1 x 1000
-// 8.5 us.
+// bound it (lengths, queries, copies, join): 8 x 3000 tokens 13.9 us, 1 x 1000
+// 8.9 us.
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"
@@ -316,10 +316,10 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
             lim[u] = p < pairs ? kv_limit(a, q, p / G) : 0;
         }
         float m[U], l[U], o[NT][4];
-        float zv[U];  // the largest z + ev so far (kv_unit)
-        int E[U];     // o is in units of 2^(E - 15)
+        float t[U];  // o is in units of 2^(E - 15), E = kv_unit(t)
+        int E[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) m[u] = zv[u] = -INFINITY, E[u] = kNoUnit, l[u] = 0.f;
+        for (int u = 0; u < U; u++) m[u] = t[u] = -INFINITY, E[u] = kNoUnit, l[u] = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -388,8 +388,8 @@ __global__ void __launch_bounds__(AW * 32, kCtasPerSm) k_kv_attn(const __grid_co
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.f : mn;
                 corr[u] = kv_ex2(m[u] - ms);
-                zv[u] = fmaxf(zv[u], mx + ev);
-                const int En = kv_unit(zv[u], ms, mx > -INFINITY ? ev : -INFINITY, E[u]);
+                t[u] = fmaxf(kv_unit_log(t[u], m[u], ms, mx, ev), mx > -INFINITY ? ev - kUnitSpan : -INFINITY);
+                const int En = kv_unit(t[u]);
                 step[u] = E[u] - En;
                 const float2 inv = kv_pow2_pair(15 - En);
                 const float up = sc.y * inv.x * inv.y;
@@ -689,8 +689,10 @@ AttnPlan plan_kv(const KvAttnCall& a, int num_sms)
     p.pt = pairs <= 8 ? 8 : 16;
     p.tiles = (int)((pairs + p.pt - 1) / p.pt);
     // 17 to 32 pairs also run here, as two tiles side by side, over short caches: k_kv_prompt takes about 8 us more to begin
-    // and end, but 25 % less per block (28 heads over 4, 4 rows: 13.6 us against 22.2 us over 512 blocks, 35.1 us against
-    // 31.2 us over 4096).  The lengths being unknown here, the capacity stands for them.
+    // and end, but less per block (28 heads over 4, 4 rows).  One sequence: 13.7 us against 21.9 us over 512 blocks, 21.3
+    // against 30.4 over 2048, 29.2 against 39.1 over 4096.  Eight: 23.6 against 17.7 over 1024, 36.6 against 31.4 over 4096;
+    // four over 2048: 31.7 against 23.4.  (From four sequences on the join goes by one CTA per (head, sequence), which costs
+    // more than the bound here allows for.)  The lengths being unknown here, the capacity stands for them.
     const int64_t blocks = (int64_t)a.c.S * a.c.H * a.c.nb;
     p.prompt = pairs > 16 && (pairs > 32 || blocks > kSideBySide);  // (two tiles is what k_kv_weights takes)
     p.runs = std::max(1, kCtasPerSm * num_sms / p.tiles);

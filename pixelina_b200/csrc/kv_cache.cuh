@@ -175,19 +175,20 @@ __device__ __forceinline__ int kv_exponent(float x) { return (int)(__float_as_ui
 // with 2^E at least the row's largest p dv so far among the blocks that it
 // sees (p relative to its running max): a block that a row may not see, or to
 // which it gives next to no weight, takes no bits from the others.
-// w: the largest z + ev of these blocks (z a block's largest score, dv < 2^ev);
-// ms: the running max, 0 if -inf; top: the largest ev among those of them that
-// come new; E: the unit so far, kNoUnit at first.  E is never below top - 111,
-// so that dv over the unit stays below 2^127 whatever the p: a row that sees blocks whose
-// scales differ by more than 2^128 loses bits of the lesser ones.  Scores of
-// 2^20 and more leave too few bits to add ev to: their unit goes by dv alone.
-constexpr int kNoUnit = -237;  // (15 - E stays below 253)
-__device__ __forceinline__ int kv_unit(float w, float ms, float top, int E)
+// E = kv_unit(t), t that p dv's log2, dv rounded up to 2^ev: kept relative to the
+// running max, so that large scores leave it its bits, and never below a seen
+// block's ev - kUnitSpan, so that dv over the unit stays below 2^127 whatever the p
+// (a row that sees blocks whose scales differ by more than 2^128 loses bits of the lesser ones).
+constexpr int kNoUnit = -237;  // nothing seen yet; 15 - E stays below 253
+constexpr float kUnitSpan = 111.f;
+__device__ __forceinline__ int kv_unit(float t) { return max(kNoUnit, __float2int_ru(t)); }
+// t behind a block of largest score z (-inf: not seen) and scale exponent ev, the
+// running max having gone from `was` to `now` (0 where it is still -inf)
+__device__ __forceinline__ float kv_unit_log(float t, float was, float now, float z, float ev)
 {
-    if (fabsf(ms) >= 1048576.f) return max(E, __float2int_ru(top));
-    return max(kNoUnit, __float2int_ru(fmaxf(w - ms, top - 111.f)));
+    return fmaxf(t - (now - was), z - now + ev);
 }
-// ev as kv_unit takes it: -inf for a NaN scale
+// ev, dv < 2^ev: -inf for a NaN scale
 __device__ __forceinline__ float kv_scale_log(float dv)
 {
     const int ev = kv_exponent(dv);

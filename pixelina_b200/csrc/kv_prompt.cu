@@ -34,13 +34,17 @@
 // rounded to nearest.
 //
 // What bounds it: with hi and lo, four half-precision products per element.  A
-// 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 237 us, in which
-// the tensor cores are issued 248 TFLOP (tiles on the diagonal whole): 1.04
-// PFLOP/s at the power cap (985 W, 1.81 GHz), where a plain bf16 product
-// sustains 1.38.  148 x 128 rows take 39.6 us over 2048 keys and 138.3 over
-// 8192: 2.06 us per tile of 128 keys and some 7 us to begin and end.
-// By clock64 a tile takes about 3400 cycles for 2048 of products: softmax 2900,
-// PV 1900 to 3100 after it, QK 1600 to 1900.
+// 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 244 us, in which
+// the tensor cores are issued 248 GFLOP (tiles on the diagonal whole): 1.02
+// PFLOP/s, where a plain bf16 product sustains 1.38.  No unit is full (of 2048
+// rows' cycles: tensor pipe 37 %, instruction issue 45 %, XU 21 %): a tile goes
+// through a chain, scores, maximum, probabilities, PV, which two softmax warps
+// per SM quarter do not hide, and a CTA takes some 7 us to begin and end.  The
+// power cap (985 W) takes the clock to 1.81 GHz of 1.965.
+// 148 x 128 rows take 39.7 us over 2048 keys and 136.9 over 8192: 2.03 us per
+// tile of 128 keys.  By clock64, before each row had its own unit (2 % since): about
+// 3400 cycles a tile for 2048 of products; softmax 2900, PV 1900 to 3100 after
+// it, QK 1600 to 1900.
 // The roles' loops are kept short: unrolled over a tile they did not fit the
 // instruction caches together, and warps waited for instructions (123 -> 93 us
 // for 148 x 128 rows over 4096 keys, together with the sums' warpgroup and the
@@ -147,8 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
     __shared__ uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2], bar_raw[2], bar_raw_empty[2], bar_s[2], bar_m[2], bar_w[2], bar_p[2][2], bar_o_full[2],
         bar_o_empty, bar_rows, bar_q, bar_fin;
     __shared__ float row_max[2][kTileRows], row_sum[2][kTileRows], row_gain[4][kTileRows];  // by tile's parity; gain by tile % 4
-    __shared__ float row_zv[2][kTileRows];  // largest z + ev so far and unit (kv_unit), by tile's parity
-    __shared__ int row_unit[2][kTileRows];
+    __shared__ float row_log[2][kTileRows];  // the rows' units (kv_unit), by tile's parity
     __shared__ float col_sum[W ? 2 : 1][2][4][kTileKeys];  // by tile's parity, alternating
     __shared__ uint32_t tmem_slot, abort_flag;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             }
         } else {
         float m = -INFINITY, l = 0.f;  // over this parity's tiles, m with the other's before it
-        int E = kNoUnit;               // P_i holds p dv / 2^(E - 15)
+        float t = -INFINITY;           // P_i holds p dv / 2^(kv_unit(t) - 15)
         for (int i = X; i < n; i += 2) {
             const int key0 = (t0 + i) * kTileKeys;
             const float2 sc = next;
@@ -350,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             if (!mbar_wait(&bar_s[X], (i >> 1) & 1, &abort_flag, status, kDevTimeoutTmemFull)) break;
             tc_fence_after();
             const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
-            float mt = -INFINITY, wt = -INFINITY, et = -INFINITY;  // the tile's largest z, z + ev, ev
+            float mt = -INFINITY, tt = -INFINITY, et = -INFINITY;  // the tile's max, its t relative to that, its largest ev
             // TMEM loads run one chunk of 16 tokens ahead of their use
             auto maxima = [&](auto masked) {
                 uint32_t r[2][16];
@@ -366,9 +369,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                         for (int c = 0; c < 16; c += 2) {
                             float x0 = __uint_as_float(r[u][c]), x1 = __uint_as_float(r[u][c + 1]);
                             if (decltype(masked)::value) {
-                                const int t = key0 + 32 * j + 16 * u + c;
-                                if (t >= lim) x0 = -INFINITY;
-                                if (t + 1 >= lim) x1 = -INFINITY;
+                                const int key = key0 + 32 * j + 16 * u + c;
+                                if (key >= lim) x0 = -INFINITY;
+                                if (key + 1 >= lim) x1 = -INFINITY;
                             }
                             mx = max3(mx, x0, x1);
                         }
@@ -376,9 +379,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                     const float k = coef * __shfl_sync(0xffffffffu, sc.x, j);
                     const float ev = __shfl_sync(0xffffffffu, evs, j);
                     if (!decltype(masked)::value || mx != -INFINITY) {
-                        mt = fmaxf(mt, mx * k);
-                        wt = fmaxf(wt, mx * k + ev);
+                        const float z = mx * k, mb = fmaxf(mt, z);
+                        tt = kv_unit_log(tt, mt, mb, z, ev);
                         et = fmaxf(et, ev);
+                        mt = mb;
                     }
                 }
                 tmem_ld_wait_dep(r[0]);
@@ -386,22 +390,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             if (full) maxima(std::false_type{});
             else maxima(std::true_type{});
             // the max and the unit of the tiles before, from the other parity
-            float mp = -INFINITY, wp = -INFINITY;
-            int Ep = kNoUnit;
+            float mp = -INFINITY, tp = -INFINITY;
             if (i > 0) {
                 if (!mbar_wait(&bar_m[X ^ 1], ((i - 1) >> 1) & 1, &abort_flag, status, kDevTimeoutScaleFull)) break;
                 mp = row_max[X ^ 1][row];
-                wp = row_zv[X ^ 1][row];
-                Ep = row_unit[X ^ 1][row];
+                tp = row_log[X ^ 1][row];
             }
             const float mn = fmaxf(mp, mt), ms = mn == -INFINITY ? 0.f : mn;
-            wt = fmaxf(wt, wp);
-            E = kv_unit(wt, ms, et, Ep);
+            t = fmaxf(fmaxf(tp - (ms - mp), tt - (ms - mt)), et - kUnitSpan);
             row_max[X][row] = mn;
-            row_zv[X][row] = wt;
-            row_unit[X][row] = E;
+            row_log[X][row] = t;
             mbar_arrive(&bar_m[X]);
-            row_gain[i & 3][row] = kv_unit_step(kv_ex2(mp - ms), Ep - E);
+            const int E = kv_unit(t);
+            row_gain[i & 3][row] = kv_unit_step(kv_ex2(mp - ms), kv_unit(tp) - E);
             const float2 inv = kv_pow2_pair(15 - E);
             l *= kv_ex2(m - ms);
             m = mn;
@@ -425,9 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                             p1 = kv_ex2(p1);
                             fmul2(y0, y1, p0, p1, y, y);
                             if (decltype(masked)::value) {
-                                const int t = key0 + 32 * j + 16 * u + 2 * c;
-                                if (t >= lim) p0 = y0 = 0.f;
-                                if (t + 1 >= lim) p1 = y1 = 0.f;
+                                const int key = key0 + 32 * j + 16 * u + 2 * c;
+                                if (key >= lim) p0 = y0 = 0.f;
+                                if (key + 1 >= lim) p1 = y1 = 0.f;
                             }
                             ffma2(add0, add1, p0, p1, 1.f, 1.f);
                             kv_split(y0, y1, hi[c], lo[c]);
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
         }
         row_max[X][row] = m;  // (read by nobody but the sums' warps any more)
         row_sum[X][row] = l;
-        row_unit[X][row] = E;
+        row_log[X][row] = t;
         named_bar_sync(1, 384);
         }
     } else if (warp < 12) {
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 P.lse[(int64_t)(q.row0 + p / G) * a.heads + h * G + p % G] = none ? INFINITY : mn + log2f(l);
             }
             const float scale = none || l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-            const float back = kv_unit_value(row_unit[(n - 1) & 1][row]);
+            const float back = kv_unit_value(kv_unit(row_log[(n - 1) & 1][row]));
             // every product is done: the row goes through smem, out by one bulk copy (or, unaligned, plain stores)
             float* dst = P.splits > 1 ? part + 2 * kTileRows + (int64_t)row * D : a.out + (int64_t)(q.row0 + p / G) * a.ldo + (int64_t)(h * G + p % G) * D;
             if (P.splits > 1 || a.ovec) {

@@ -143,3 +143,29 @@ def test_a_hidden_block_in_a_ragged_batch(pxq):
     for s in range(3):
         want, _ = ref.attention(q[2 * s:2 * s + 2], ref.values(b.k[s]), ref.values(b.v[s]), heads, True)
         assert_rows_close(got[2 * s:2 * s + 2], want)
+
+
+@pytest.mark.parametrize("rows,group", ROWS[:4])
+@pytest.mark.parametrize("up", [18, 24, 40])
+def test_scores_beyond_what_a_softmax_can_tell_apart(pxq, rows, group, up):
+    """Scores of 2^up and more, the blocks' values of very different scale: every row takes the value of its best token (the
+    next one is 2^(up - 8) below it or more; a tenth of the rows, with a nearer one, is left out)."""
+    D, t, H = 64, 1536, kv_heads(rows)
+    rng = np.random.default_rng(up)
+    k = rows_of(rng, t, H, D, 0.0)
+    v = (rng.standard_normal((t, H, D)) * 2.0 ** (30 * np.sin(np.arange(t) // 32))[:, None, None]).astype(np.float32)
+    q = (2.0 ** up * rng.standard_normal((rows, H * group, D))).astype(np.float32)
+    got = pxq.kv_attention(dev(q.reshape(rows, -1)), filled(pxq, k, v, H, D), H * group, causal=False).cpu().numpy().reshape(rows, H * group, D)
+    pxq.synchronize()
+    kv, vv = ref.values(k).astype(np.float64), ref.values(v)
+    for h in range(H):
+        left = 0
+        for i in range(rows):
+            for g in range(h * group, (h + 1) * group):
+                z = kv[:, h] @ q[i, g].astype(np.float64) / np.sqrt(D)
+                second, best = np.partition(z, -2)[-2:]
+                if best - second < 2.0 ** (up - 8):
+                    left += 1
+                    continue
+                assert_rows_close(got[i, g], vv[z.argmax(), h].astype(np.float64))
+        assert left <= 2 + 0.1 * rows * group
