@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(AW * 32, PT == 8 ? 3 : 2) k_kv_weights(const _
             for (int i = 0; i < 8; i++)
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    w[i] += t0 + i < lim[tile][u] ? kv_ex2(z[u][i] * (qf[tile].coef[u] * dk) - lse[tile][u]) : 0.f;
+                    w[i] += t0 + i < lim[tile][u] ? kv_ex2(__fmul_rn(z[u][i], qf[tile].coef[u] * dk) - lse[tile][u]) : 0.f;
         }
         // each step adds two rows and halves the tokens that a lane holds: lane (r, c) ends up with token 8 c + r
 #pragma unroll

@@ -108,6 +108,12 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
+// Up to here a score's product and its distance from the max may be one fused
+// step.  Above, the max being a rounded product, the unrounded one can exceed it by
+// so much that p would leave fp16's range: those tiles take the rounded products,
+// like those with masks.
+constexpr float kFusedScores = 1048576.f;
+
 struct PromptParams {
     KvAttnCall a;
     float* part;  // splits > 1: [split][tile][head]: planes m[128], l[128], (O / l)[128][D]
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 tc_fence_after();
                 const bool full = __all_sync(0xffffffffu, key0 + kTileKeys <= lim);
                 float* const cols = col_sum[X][(i >> 1) & 1][warp & 3];
-                auto add_up = [&](auto masked) {
+                auto add_up = [&](auto careful) {
 #pragma unroll 1
                     for (int j = 0; j < 4; j++) {
                         uint32_t r[32];
@@ -311,10 +317,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
                             float p0 = -lse, p1 = -lse;
-                            ffma2(p0, p1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k, k);
+                            if (decltype(careful)::value) {
+                                p0 += __fmul_rn(__uint_as_float(r[c]), k);
+                                p1 += __fmul_rn(__uint_as_float(r[c + 1]), k);
+                            } else {
+                                ffma2(p0, p1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k, k);
+                            }
                             w[c] = kv_ex2(p0);
                             w[c + 1] = kv_ex2(p1);
-                            if (decltype(masked)::value) {
+                            if (decltype(careful)::value) {
                                 const int t = key0 + 32 * j + c;
                                 if (t >= lim) w[c] = 0.f;
                                 if (t + 1 >= lim) w[c + 1] = 0.f;
@@ -333,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                         cols[32 * j + lane] = w[0];
                     }
                 };
-                if (full) add_up(std::false_type{});
+                if (full && __all_sync(0xffffffffu, fabsf(lse) < kFusedScores)) add_up(std::false_type{});
                 else add_up(std::true_type{});
                 tc_fence_before();
                 mbar_arrive(&bar_p[X][0]);
@@ -407,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
             l *= kv_ex2(m - ms);
             m = mn;
             float add0 = 0.f, add1 = 0.f;
-            auto weigh = [&](auto masked) {
+            auto weigh = [&](auto careful) {
                 uint32_t r[2][16];
                 tmem_ld16(ts, r[0]);
 #pragma unroll 1
@@ -421,11 +432,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
 #pragma unroll
                         for (int c = 0; c < 8; c++) {
                             float p0 = -ms, p1 = -ms, y0, y1;
-                            ffma2(p0, p1, __uint_as_float(r[u][2 * c]), __uint_as_float(r[u][2 * c + 1]), k, k);
+                            if (decltype(careful)::value) {
+                                p0 += __fmul_rn(__uint_as_float(r[u][2 * c]), k);
+                                p1 += __fmul_rn(__uint_as_float(r[u][2 * c + 1]), k);
+                            } else {
+                                ffma2(p0, p1, __uint_as_float(r[u][2 * c]), __uint_as_float(r[u][2 * c + 1]), k, k);
+                            }
                             p0 = kv_ex2(p0);
                             p1 = kv_ex2(p1);
                             fmul2(y0, y1, p0, p1, y, y);
-                            if (decltype(masked)::value) {
+                            if (decltype(careful)::value) {
                                 const int key = key0 + 32 * j + 16 * u + 2 * c;
                                 if (key >= lim) p0 = y0 = 0.f;
                                 if (key + 1 >= lim) p1 = y1 = 0.f;
@@ -444,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_prompt(const __grid_constant
                 }
                 tmem_ld_wait_dep(r[0]);
             };
-            if (full) weigh(std::false_type{});
+            if (full && __all_sync(0xffffffffu, fabsf(ms) < kFusedScores)) weigh(std::false_type{});
             else weigh(std::true_type{});
             l += add0 + add1;
         }

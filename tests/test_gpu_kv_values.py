@@ -145,7 +145,7 @@ def test_a_hidden_block_in_a_ragged_batch(pxq):
         assert_rows_close(got[2 * s:2 * s + 2], want)
 
 
-@pytest.mark.parametrize("rows,group", ROWS[:4])
+@pytest.mark.parametrize("rows,group", ROWS)
 @pytest.mark.parametrize("up", [18, 24, 40])
 def test_scores_beyond_what_a_softmax_can_tell_apart(pxq, rows, group, up):
     """Scores of 2^up and more, the blocks' values of very different scale: every row takes the value of its best token (the
@@ -155,11 +155,12 @@ def test_scores_beyond_what_a_softmax_can_tell_apart(pxq, rows, group, up):
     k = rows_of(rng, t, H, D, 0.0)
     v = (rng.standard_normal((t, H, D)) * 2.0 ** (30 * np.sin(np.arange(t) // 32))[:, None, None]).astype(np.float32)
     q = (2.0 ** up * rng.standard_normal((rows, H * group, D))).astype(np.float32)
-    got = pxq.kv_attention(dev(q.reshape(rows, -1)), filled(pxq, k, v, H, D), H * group, causal=False).cpu().numpy().reshape(rows, H * group, D)
+    w = dev(np.zeros((1, H, t), np.float32))
+    got = pxq.kv_attention(dev(q.reshape(rows, -1)), filled(pxq, k, v, H, D), H * group, causal=False, weights_out=w).cpu().numpy().reshape(rows, H * group, D)
     pxq.synchronize()
-    kv, vv = ref.values(k).astype(np.float64), ref.values(v)
+    kv, vv, w = ref.values(k).astype(np.float64), ref.values(v), w[0].cpu().numpy()
     for h in range(H):
-        left = 0
+        left, count = 0, np.zeros(t)
         for i in range(rows):
             for g in range(h * group, (h + 1) * group):
                 z = kv[:, h] @ q[i, g].astype(np.float64) / np.sqrt(D)
@@ -167,5 +168,7 @@ def test_scores_beyond_what_a_softmax_can_tell_apart(pxq, rows, group, up):
                 if best - second < 2.0 ** (up - 8):
                     left += 1
                     continue
+                count[z.argmax()] += 1
                 assert_rows_close(got[i, g], vv[z.argmax(), h].astype(np.float64))
         assert left <= 2 + 0.1 * rows * group
+        assert np.abs(w[h] - count).sum() <= left * 1.01 + ATT_TOL * rows * group
