@@ -358,9 +358,6 @@ def _whole(x, shape, dtype, what: str, device):
     return x.data_ptr()
 
 
-_PER_THREAD_STREAM = 2  # cudaStreamPerThread
-
-
 class KVCache:
     """An 8-bit key/value cache (pxq_kv_cache) for `sequences` sequences of up
     to `capacity` tokens; its memory is a torch tensor of its own."""
@@ -383,16 +380,11 @@ class KVCache:
 
     def release(self) -> None:
         """Forget the cache; its memory goes back to torch, which hands it out
-        again when every stream that worked on it is done."""
+        again when every stream that worked on it is done.  (cudaStreamPerThread
+        is another stream in every thread, and torch only knows the releasing one's: wait for the others first.)"""
         if self.handle:
-            self._settle()
             _check(load().pxq_kv_cache_release(self.handle))
             self.handle, self.memory = C.c_void_p(), None
-
-    def _settle(self):
-        # the per-thread stream's handle is another stream in every thread: torch could only wait for this thread's
-        if _PER_THREAD_STREAM in self._streams:
-            _torch().cuda.synchronize(self.device)
 
     def _on_stream(self, stream):
         """Address of the stream that a call runs on, which torch is told of where the memory is another stream's."""
@@ -404,7 +396,6 @@ class KVCache:
 
     def __del__(self):
         if getattr(self, "handle", None) and _lib is not None:
-            self._settle()
             _lib.pxq_kv_cache_release(self.handle)
             self.handle = C.c_void_p()
 
@@ -436,7 +427,8 @@ class KVCache:
                                     self._on_stream(stream)))
 
     def truncate(self, lengths=None, stream=None) -> None:
-        """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them)."""
+        """Shorten the sequences to `lengths` (int32 cuda tensor; None: empty them).
+        Running totals of weights stay: set those of the dropped tokens to zero."""
         _check(load().pxq_kv_truncate(self._live(), self._per_sequence(lengths, "lengths"), self._on_stream(stream)))
 
     def read(self, first=None, count: Optional[int] = None, k=None, v=None, stream=None):
@@ -460,7 +452,7 @@ def kv_attention(q, cache: KVCache, heads: int, starts=None, max_rows: Optional[
                  weights_out=None, out=None, stream=None):
     """Attention of q [rows, heads*d] over the cache (pxq_kv_attention): rows
     [starts[s], starts[s+1]) are sequence s's, at most max_rows of them each
-    (None: no bound but rows).  weights_out = weights + what each cached token
+    (None: no bound but rows, which plans for a prompt).  weights_out = weights + what each cached token
     received, [sequences, kv_heads, capacity]."""
     torch = _torch()
     h, device = cache._live(), cache.device

@@ -215,3 +215,32 @@ def test_a_token_taken_back_and_appended_again(pxq):
         after = b.cache.memory
         assert bool((before[:512 + scales] == after[:512 + scales]).all()) and bool((before[-codes:] == after[-codes:]).all())
     pxq.synchronize()
+
+
+def test_drafts_taken_back_with_their_weights(pxq):
+    """A rejected draft: the cache shortened and the dropped tokens' running totals set to zero, as the interface asks; later
+    steps then add up to what they would without the draft."""
+    import torch
+
+    rng = np.random.default_rng(31)
+    H, D, heads, t, cap = 2, 64, 8, 50, 80
+    x = [dev(rows_of(rng, n, H, D).reshape(n, -1)) for n in (t, 5, 3)]
+    qs = [dev(rng.standard_normal((n, heads * D)).astype(np.float32)) for n in (1, 5, 3)]
+    totals = []
+    for draft in (False, True):
+        cache, w = pxq.KVCache(1, cap, H, D), torch.zeros((1, H, cap), device="cuda")
+        cache.append(x[0], x[0])
+        pxq.kv_attention(qs[0], cache, heads, weights=w, weights_out=w)
+        if draft:
+            seen = w.clone()
+            cache.append(x[1], x[1])
+            pxq.kv_attention(qs[1], cache, heads, weights=w, weights_out=w)
+            assert bool((w[:, :, t:t + 5] > 0).all())
+            cache.truncate(i32([t]))
+            w.copy_(seen)  # what the draft gave to the tokens before it goes too
+            w[:, :, t:] = 0
+        cache.append(x[2], x[2])
+        pxq.kv_attention(qs[2], cache, heads, weights=w, weights_out=w)
+        totals.append(w)
+    pxq.synchronize()
+    assert torch.equal(*totals)

@@ -34,29 +34,3 @@ def test_memory_is_not_handed_out_while_another_stream_works_on_it(pxq, how, cur
     assert other.data_ptr() != at
     side.synchronize()
     pxq.synchronize()
-
-
-def test_released_after_use_on_the_per_thread_stream(pxq):
-    """One handle for as many streams as there are threads: the release waits for them all."""
-    import threading
-
-    import torch
-
-    side = torch.cuda.ExternalStream(2)
-    x = torch.ones((70, 128), device="cuda")
-    cache = pxq.KVCache(1, 1000, 2, 64)
-    torch.cuda.synchronize()
-    done = torch.cuda.Event()
-
-    def work():
-        with torch.cuda.stream(side):
-            torch.cuda._sleep(200_000_000)
-            cache.append(x, x)
-            done.record()
-
-    t = threading.Thread(target=work)
-    t.start()
-    t.join()
-    cache.release()
-    assert done.query()
-    pxq.synchronize()

@@ -92,34 +92,32 @@ def test_threads_on_one_stream(pxq):
         assert all(torch.equal(got, x) for got, x in zip(c.results(), w))
 
 
-def test_threads_on_their_per_thread_streams(pxq):
-    """cudaStreamPerThread is one handle for as many streams as there are threads."""
+def test_the_per_thread_stream(pxq):
+    """cudaStreamPerThread is one handle for as many streams as there are threads, so its calls have scratch of their own; here
+    from one thread, the results those of the default stream."""
     import torch
 
     per_thread = torch.cuda.ExternalStream(2)
-    mine = chats(pxq, (per_thread,) * 3)
+    results = []
+    for stream in (None, per_thread):
+        mine = chats(pxq, (stream,) * 3)
+        torch.cuda.synchronize()
+        for c in mine:
+            for i in range(Chat.KEEP):
+                c.step(i)
+        torch.cuda.synchronize()
+        results.append([x for c in mine for x in c.results()])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    W = pxq.Weight(synth.random_q5_K(200, 2048, np.random.default_rng(1)), 13, 2048, 200)
+    x = dev(synth.activations(8, 2048, seed=6))
     torch.cuda.synchronize()
-    for c in mine:
-        for i in range(Chat.KEEP):
-            c.step(i)
-    pxq.synchronize(per_thread)
-    want = [c.results() for c in mine]
-    for c in mine:
-        c.clear()
+    with torch.cuda.stream(per_thread):
+        got = [pxq.matmul(W, x) for _ in range(4)]
+        per_thread.synchronize()
+    want = pxq.matmul(W, x)
     torch.cuda.synchronize()
-
-    def work(c):
-        def step(i):
-            c.step(i)
-            if i % Chat.KEEP == Chat.KEEP - 1:
-                pxq.synchronize(per_thread)
-        return step
-
-    together([work(c) for c in mine])
-    torch.cuda.synchronize()
-    for c, w in zip(mine, want):
-        assert all(torch.equal(got, x) for got, x in zip(c.results(), w))
-    pxq.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    W.release()
 
 
 def test_threads_share_a_stream_with_older_calls(pxq):
