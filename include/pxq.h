@@ -7,7 +7,10 @@
  * pinned) host memory.  Streams are passed as `void*` holding a cudaStream_t
  * (NULL = the legacy default stream).  All functions return PXQ_OK (0) or a
  * PXQ_ERR_* code; pxq_last_error() gives a one-line description for the
- * calling thread.
+ * calling thread.  Host threads may call at once, on streams of their own, on
+ * one that they share, or on cudaStreamPerThread (a thread that ends waits for
+ * its own first): a call's kernels follow each other on its stream, no other
+ * call's in between over the same scratch.
  *
  * Layout conventions follow the reference (paths are within the Pixelina
  * source tree):
@@ -446,7 +449,10 @@ PXQ_API int pxq_kv_append(pxq_kv_cache* c, const float* k, size_t ldk, const flo
 /* Shorten every sequence s to lengths[s] tokens (device int32; NULL: 0).  A
  * value that is negative or not below the present length leaves the sequence
  * as it is.  Going back within the last block is exact; a block that was
- * closed is opened again from the values it stands for. */
+ * closed is opened again from the values it stands for.  Running totals of
+ * attention weights are the caller's: those of the dropped tokens stay, and
+ * tokens that are appended in their place add to them, unless the caller sets
+ * them to zero. */
 PXQ_API int pxq_kv_truncate(pxq_kv_cache* c, const int32_t* lengths, void* stream);
 
 /* The values the cache stands for: tokens [first[s], first[s] + count) of
@@ -465,10 +471,16 @@ PXQ_API int pxq_kv_read(const pxq_kv_cache* c, const int32_t* first, size_t coun
  * len - n + i + 1 of them; otherwise every row sees all len.  A row that sees
  * nothing gets zeros.  Rows of a sequence with bounds outside the arrays or more
  * than max_rows rows are not written (a device-side error, as above).
+ * max_rows and the capacity choose the kernels for the whole batch, the
+ * lengths being unknown here: give the bound that holds (with a looser one, single
+ * tokens take the prompts' route), and call twice where a few long prompts
+ * come with single tokens over long caches, each time with bounds that leave
+ * the other sequences without rows.
  * weights_out (may be NULL): [sequences][kv_heads][capacity], the attention
  * weight that each cached token received from the rows and the heads that
  * share its kv head, added to `weights` (same shape; NULL: zeros; may be
- * weights_out itself).  Entries past a sequence's length are not touched.
+ * weights_out itself; from scores of 2^20 and more, good to the scores' own
+ * fp32 spacing).  Entries past a sequence's length are not touched.
  * heads must be a multiple of the cache's kv_heads; output may not overlap q. */
 PXQ_API int pxq_kv_attention(const pxq_kv_cache* c, const float* q, size_t ldq, size_t rows, const int32_t* starts,
                              size_t max_rows, size_t heads, int causal, float* output, size_t ldo, const float* weights,

@@ -22,13 +22,13 @@
 //   k_kv_weights  the weights, from each pair's max and sum
 //
 // What bounds k_kv_attn: reading the cache once, 2 len D bytes per (sequence,
-// head).  8 x 49000 tokens, 28 heads over 4 of 128: 71.6 us, 5.6 TB/s of 6.5.
+// head).  8 x 49000 tokens, 28 heads over 4 of 128: 70.9 us, 5.7 TB/s of 6.5.
 // Per block of 32 tokens a warp has 64 products (8 cycles each and SM
 // quarter) and, counted in the source, some 470 instructions, about half of
 // them turning codes into fp16; the registers leave room for two warps per
 // quarter.  With little to read the two kernels' chains of dependent steps
-// bound it (lengths, queries, copies, join): 8 x 3000 tokens 13.9 us, 1 x 1000
-// 8.9 us.
+// bound it (lengths, queries, copies, join): 8 x 3000 tokens 13.8 us, 1 x 1000
+// 8.7 us.
 #include <algorithm>
 #include <type_traits>
 #include "kv_cache.cuh"

@@ -34,14 +34,14 @@
 // rounded to nearest.
 //
 // What bounds it: with hi and lo, four half-precision products per element.  A
-// 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 244 us, in which
-// the tensor cores are issued 248 GFLOP (tiles on the diagonal whole): 1.02
+// 4096-token prompt of 28 heads over 4 (D = 128, causal) takes 248 us, in which
+// the tensor cores are issued 248 GFLOP (tiles on the diagonal whole): 1.00
 // PFLOP/s, where a plain bf16 product sustains 1.38.  No unit is full (of 2048
-// rows' cycles: tensor pipe 37 %, instruction issue 45 %, XU 21 %): a tile goes
+// rows' cycles: tensor pipe 38 %, instruction issue 45 %, XU 21 %): a tile goes
 // through a chain, scores, maximum, probabilities, PV, which two softmax warps
-// per SM quarter do not hide, and a CTA takes some 7 us to begin and end.  The
+// per SM quarter do not hide, and a CTA takes some 8 us to begin and end.  The
 // power cap (985 W) takes the clock to 1.81 GHz of 1.965.
-// 148 x 128 rows take 39.7 us over 2048 keys and 136.9 over 8192: 2.03 us per
+// 148 x 128 rows take 40.6 us over 2048 keys and 137.9 over 8192: 2.03 us per
 // tile of 128 keys.  By clock64, before each row had its own unit (2 % since): about
 // 3400 cycles a tile for 2048 of products; softmax 2900, PV 1900 to 3100 after
 // it, QK 1600 to 1900.
